@@ -432,6 +432,84 @@ int32_t nomos_kv_paged_append_quant_i8(void *stream, uint64_t src_k, uint64_t sr
                                        uint64_t ks_pool, uint64_t vs_pool, uint64_t block_table, uint64_t positions,
                                        int32_t batch, int32_t nkv, int32_t l_hd, int32_t l_kvd, int32_t max_pages);
 
+/* ---- A serving step on paged caches, from request lengths to accepted tokens (no counterpart in the reference, which
+ * serves one sequence; its verify step compares argmax rows on the host, pyhost/host.py:212-218).  Lengths, tables, slots
+ * and tokens stay on the GPU, every launch has a size the host knows beforehand, so that a step can be captured:
+ *   nomos_kv_paged_plan            pages, slots and positions of the step's rows
+ *   nomos_kv_paged_append_rows_i8  the rows into their slots, bounds of the pages they complete
+ *   nomos_attn_paged_sparse_i8     attention of every row over the pages its bounds select (top_pages >= the sequence's
+ *                                  pages: over all of them)
+ *   nomos_attn_spec_verify         drafted tokens against the target's probabilities, lengths advanced
+ * Integer arrays are int32.
+ *
+ * Block tables and slot maps.  Request b has seq_lens[b] keys cached, brings n_new[b] rows and holds held[b] pages, the first
+ * held[b] entries of its row of block_table [batch][max_pages].  free_pages [n_pages] is a stack of free_count[0] page numbers.
+ *   n_new[b] < 0: the request is finished; its pages go back onto the stack (requests in order, each one's pages in order)
+ *     before any are handed out.  0: nothing happens.
+ *   n_new[b] > 0: the request lacks ceil((seq_lens + n_new) / 128) - held pages.  Pages are taken from the top of the stack,
+ *     requests in order.  From the first request on whose pages the stack no longer covers, no request is given any (one that
+ *     lacks none is still served); neither is served a request whose keys exceed max_pages * 128 or whose rows end behind
+ *     max_rows.
+ * Written: block_table (new entries), free_pages (released pages), held_out, free_count_out, granted[b] (rows placed: n_new or
+ * 0), row_start [batch + 1] (first row of each request, at most max_rows), and for each of the max_rows rows slot_map
+ * (page * 128 + position % 128), row_seq and row_pos: -1 in all three behind the last request and for rows not granted.
+ * held_out may be held and free_count_out free_count (one step after another, or a captured graph replayed); with arrays of
+ * their own a plan can be dropped: the entries it wrote lie behind what held and free_count count.  seq_lens is not written:
+ * add what was kept (nomos_attn_spec_verify does), so rows rejected there are planned again, into the pages already held.
+ * At most 8192 requests. */
+int32_t nomos_kv_paged_plan(void *stream, uint64_t seq_lens, uint64_t n_new, uint64_t held, uint64_t free_pages, uint64_t free_count,
+                            uint64_t block_table, uint64_t held_out, uint64_t free_count_out, uint64_t granted, uint64_t row_start,
+                            uint64_t slot_map, uint64_t row_seq, uint64_t row_pos, int32_t batch, int32_t max_pages, int32_t n_pages,
+                            int32_t max_rows);
+/* Quantising append of n_rows rows (src [n_rows][nkv][l_hd] of src_type, row stride l_kvd elements) into slots slot_map[r] of
+ * the pools, with the row codec of nomos_kv_append_quant_i8.  Slots outside the pool (-1: padding) are skipped; a slot may
+ * occur once.  With kb_pool and kbs_pool (else both 0) the bounds of each page whose row 127 is among the slots are computed
+ * once all rows are in: kb_pool [n_pages][nkv][2][128] int8 (16-byte aligned), kbs_pool [n_pages][nkv] fp32.  With v the page's
+ * dequantised keys, per channel the largest and the smallest, divided by t = (largest magnitude) / 127 and rounded up and
+ * down: t * kb[0] >= v >= t * kb[1] up to one rounding.  A page with a row scale that is not finite gets t = +inf, codes 0. */
+int32_t nomos_kv_paged_append_rows_i8(void *stream, uint64_t src_k, uint64_t src_v, uint64_t k_pool, uint64_t v_pool, uint64_t ks_pool,
+                                      uint64_t vs_pool, uint64_t kb_pool, uint64_t kbs_pool, uint64_t slot_map, int32_t n_rows,
+                                      int32_t nkv, int32_t l_hd, int32_t l_kvd, int32_t n_pages, int32_t src_type);
+/* The same bounds for n listed pages (entries outside the pool are skipped): for pages filled by
+ * nomos_kv_paged_append_quant_i8 or copied in. */
+int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks_pool, uint64_t kb_pool, uint64_t kbs_pool, uint64_t pages,
+                                      int32_t n, int32_t nkv, int32_t l_hd, int32_t n_pages);
+/* Attention of `rows` query rows (q, out [rows][nh][128]) over selected pages.  Row r is position row_pos[r] of sequence
+ * row_seq[r]; it sees keys 0 .. row_pos[r] of the pages selected for it, per KV head.  Rows with row_seq outside [0, batch) or
+ * row_pos outside [0, max_len) are skipped, their part of out and sel_pages left as it is.
+ * A row with P = row_pos / 128 + 1 <= top_pages pages reads all of them.  Otherwise: the first sink_pages, the last
+ * local_pages (its own among them) and the best of the others by  score = max over the group's heads of
+ * (t * sum_d max(q^_d kb[0][d], q^_d kb[1][d])) * s, where q^, s is the head's query in the int8 row codec (elements that are
+ * not finite count 0): up to the query's rounding the largest logit any key of the page can have.  Equal scores: the lower page.  The sum is
+ * a whole number and exact, the two products are rounded to binary32, so the selection is reproducible to the bit; scores
+ * that are not finite count as the largest finite value (a page of NaN keys is read, as dense attention would read it).
+ * Every page but the row's last must have its bounds (see above).
+ * sel_pages: 0, or [rows][nkv][top_pages], the page numbers within the sequence in ascending order, -1 beyond.
+ * Accuracy of out: that of nomos_attn_paged_decode_i8 over the selected keys.  head_dim 128, at most 8 heads per KV head.
+ * The workspace (16-byte aligned) must not be shared by calls that can overlap on the GPU. */
+int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t top_pages,
+                                                int32_t max_len);
+int32_t nomos_attn_paged_sparse_i8(void *stream, uint64_t q, uint64_t k_pool, uint64_t v_pool, uint64_t ks_pool, uint64_t vs_pool,
+                                   uint64_t kb_pool, uint64_t kbs_pool, uint64_t block_table, uint64_t row_seq, uint64_t row_pos,
+                                   uint64_t out, uint64_t sel_pages, uint64_t workspace, int64_t ws_bytes, int32_t rows, int32_t batch,
+                                   int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t n_pages, int32_t max_pages,
+                                   int32_t max_len, int32_t top_pages, int32_t sink_pages, int32_t local_pages, double softmax_scale,
+                                   int32_t q_type, int32_t out_type);
+/* Verification of drafted tokens from given random numbers.  Sequence b drafted n_draft[b] tokens (0 pointer: max_draft each;
+ * negative: the sequence is idle and nothing of it is written; more than max_draft count as max_draft).  target_probs
+ * [batch][max_draft + 1][p_stride], draft_probs [batch][max_draft][q_stride] fp32 rows of `vocab` probabilities in [0, 1]
+ * (draft_probs 0: a drafter that gives tokens only, probability 1 each); u_accept [batch][max_draft], u_sample [batch] in [0, 1).
+ * Draft i of token x is accepted iff u_accept * q_i(x) < p_i(x), in 64 bits; a token outside [0, vocab) is rejected.  With a
+ * the first one rejected (n_draft if none): n_accepted[b] = a, out_tokens [batch][max_draft + 1] = the a accepted tokens, then
+ * one drawn from max(p_a - q_a, 0) -- from p_a where none was rejected, or where that is zero throughout -- then -1.  The draw:
+ * W_i = rint(weight_i * 2^50), T = floor(u_sample * sum W) in 64 bits, the first token with W_0 + .. + W_i > T; -1 if all are
+ * zero.  Whole-number sums make it independent of how the row is split.
+ * seq_lens_out[b] = seq_lens[b] + a + 1, the keys that stay cached once the last sampled token's row and the accepted drafts'
+ * rows are (seq_lens may be seq_lens_out; both 0: no lengths). */
+int32_t nomos_attn_spec_verify(void *stream, uint64_t target_probs, uint64_t draft_probs, uint64_t draft_tokens, uint64_t n_draft,
+                               uint64_t u_accept, uint64_t u_sample, uint64_t seq_lens, uint64_t seq_lens_out, uint64_t n_accepted,
+                               uint64_t out_tokens, int32_t batch, int32_t max_draft, int32_t vocab, int64_t p_stride, int64_t q_stride);
+
 /* ------------------------------------------------------------------------- *
  *  Sequence-sharded decode across the GPUs of one node (no counterpart in the reference, which runs on   *
  *  one GPU, lib/gemma4_engine.mojo:229)                                                                  *

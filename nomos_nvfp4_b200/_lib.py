@@ -66,6 +66,12 @@ PROTOTYPES = {
     "nomos_attn_paged_workspace_bytes": (i64, [i32] * 6),
     "nomos_attn_paged_decode_i8": (i32, [vp] + [u64] * 9 + [i64] + [i32] * 8 + [C.c_double, i32, i32]),
     "nomos_kv_paged_append_quant_i8": (i32, [vp] + [u64] * 8 + [i32] * 5),
+    "nomos_kv_paged_plan": (i32, [vp] + [u64] * 13 + [i32] * 4),
+    "nomos_kv_paged_append_rows_i8": (i32, [vp] + [u64] * 9 + [i32] * 6),
+    "nomos_kv_paged_page_bounds_i8": (i32, [vp] + [u64] * 5 + [i32] * 4),
+    "nomos_attn_paged_sparse_workspace_bytes": (i64, [i32] * 7),
+    "nomos_attn_paged_sparse_i8": (i32, [vp] + [u64] * 13 + [i64] + [i32] * 12 + [C.c_double, i32, i32]),
+    "nomos_attn_spec_verify": (i32, [vp] + [u64] * 10 + [i32] * 3 + [i64] * 2),
     "nomos_attn_fused_host": (i32, [vp, C.POINTER(AttnArgs), u64, u64, C.c_int64, u64, u64, C.c_int64]),
     "nomos_kv_norm_rope_append": (i32, [vp] + [u64] * 11 + [i32] * 8 + [C.c_float, i32, i32]),
     "nomos_kv_quant_i8": (i32, [vp, u64, u64, u64, i32, i32]),

@@ -1,5 +1,6 @@
 // extern "C" surface of libnomos_attn.so: argument validation + forwarding.
 // Declarations and per-function reference citations live in include/nomos_attn.h.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -660,6 +661,185 @@ NOMOS_EXPORT int32_t nomos_kv_paged_append_quant_i8(void *stream, uint64_t src_k
     return launch_append_paged_i8(as_stream(stream), ptr(src_k), ptr(src_v), ptr(k_pool), ptr(v_pool), ptr(ks_pool), ptr(vs_pool),
                                   static_cast<const int *>(ptr(block_table)), static_cast<const int *>(ptr(positions)), batch, nkv,
                                   l_hd, l_kvd, max_pages);
+}
+
+// ------------------------------------------------------------------- batch serving on paged caches
+
+NOMOS_EXPORT int32_t nomos_kv_paged_plan(void *stream, uint64_t seq_lens, uint64_t n_new, uint64_t held, uint64_t free_pages,
+                                         uint64_t free_count, uint64_t block_table, uint64_t held_out, uint64_t free_count_out,
+                                         uint64_t granted, uint64_t row_start, uint64_t slot_map, uint64_t row_seq, uint64_t row_pos,
+                                         int32_t batch, int32_t max_pages, int32_t n_pages, int32_t max_rows) {
+    const char *who = "nomos_kv_paged_plan";
+    if (batch <= 0) return NOMOS_OK;
+    REQUIRE(seq_lens && n_new && held && free_pages && free_count && block_table && held_out && free_count_out && granted && row_start,
+            "%s: null pointer", who);
+    REQUIRE(max_rows >= 0 && (max_rows == 0 || (slot_map && row_seq && row_pos)), "%s: null pointer or negative max_rows", who);
+    REQUIRE(max_pages > 0 && n_pages > 0, "%s: bad max_pages/n_pages", who);
+    for (uint64_t x : {seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start, slot_map,
+                       row_seq, row_pos})
+        REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);
+    REQUIRE((int64_t)max_pages * 128 < (1l << 31) && (int64_t)n_pages * 128 < (1l << 31), "%s: positions and slots are 32-bit numbers", who);
+    if (batch > PLAN_MAX_BATCH) { set_error("%s: at most %d requests per call", who, PLAN_MAX_BATCH); return NOMOS_EUNSUPPORTED; }
+    const auto in = [](uint64_t a) { return static_cast<const int *>(ptr(a)); };
+    const auto io = [](uint64_t a) { return static_cast<int *>(ptr(a)); };
+    return launch_paged_plan(as_stream(stream), in(seq_lens), in(n_new), in(held), io(free_pages), in(free_count), io(block_table), io(held_out),
+                             io(free_count_out), io(granted), io(row_start), io(slot_map), io(row_seq), io(row_pos), batch, max_pages, n_pages,
+                             max_rows);
+}
+
+static int check_page_pool(const char *who, int nkv, int l_hd, int n_pages) {
+    REQUIRE(nkv > 0 && n_pages > 0, "%s: bad nkv/n_pages", who);
+    if (l_hd != 128 || nkv > 65535) { set_error("%s: paged caches support head_dim 128", who); return NOMOS_EUNSUPPORTED; }
+    REQUIRE((int64_t)n_pages * 128 < (1l << 31), "%s: slots are 32-bit numbers", who);
+    return NOMOS_OK;
+}
+
+NOMOS_EXPORT int32_t nomos_kv_paged_append_rows_i8(void *stream, uint64_t src_k, uint64_t src_v, uint64_t k_pool, uint64_t v_pool,
+                                                   uint64_t ks_pool, uint64_t vs_pool, uint64_t kb_pool, uint64_t kbs_pool,
+                                                   uint64_t slot_map, int32_t n_rows, int32_t nkv, int32_t l_hd, int32_t l_kvd,
+                                                   int32_t n_pages, int32_t src_type) {
+    const char *who = "nomos_kv_paged_append_rows_i8";
+    if (n_rows <= 0) return NOMOS_OK;
+    REQUIRE(src_k && src_v && k_pool && v_pool && ks_pool && vs_pool && slot_map, "%s: null pointer", who);
+    REQUIRE((kb_pool != 0) == (kbs_pool != 0), "%s: page bounds need both of their pools", who);
+    int rc = check_page_pool(who, nkv, l_hd, n_pages);
+    if (rc) return rc;
+    REQUIRE((int64_t)l_kvd >= (int64_t)nkv * l_hd, "%s: rows of %d elements, %d apart", who, nkv * l_hd, l_kvd);
+    REQUIRE(src_type == ET_F32 || src_type == ET_BF16, "%s: element type", who);
+    const uint64_t es = src_type == ET_BF16 ? 2 : 4;
+    REQUIRE(aligned(src_k, es) && aligned(src_v, es) && aligned(k_pool, 16) && aligned(v_pool, 16) && aligned(ks_pool, 4) &&
+                aligned(vs_pool, 4) && aligned(kb_pool, 16) && aligned(kbs_pool, 4) && aligned(slot_map, 4), "%s: misaligned buffer", who);
+    return launch_append_slots_i8(as_stream(stream), ptr(src_k), ptr(src_v), ptr(k_pool), ptr(v_pool), ptr(ks_pool), ptr(vs_pool),
+                                  ptr(kb_pool), ptr(kbs_pool), static_cast<const int *>(ptr(slot_map)), n_rows, nkv, l_kvd, n_pages,
+                                  src_type == ET_BF16);
+}
+
+NOMOS_EXPORT int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks_pool, uint64_t kb_pool, uint64_t kbs_pool,
+                                                   uint64_t pages, int32_t n, int32_t nkv, int32_t l_hd, int32_t n_pages) {
+    const char *who = "nomos_kv_paged_page_bounds_i8";
+    if (n <= 0) return NOMOS_OK;
+    REQUIRE(k_pool && ks_pool && kb_pool && kbs_pool && pages, "%s: null pointer", who);
+    int rc = check_page_pool(who, nkv, l_hd, n_pages);
+    if (rc) return rc;
+    REQUIRE(aligned(k_pool, 16) && aligned(ks_pool, 4) && aligned(kb_pool, 16) && aligned(kbs_pool, 4) && aligned(pages, 4), "%s: misaligned buffer", who);
+    return launch_page_bounds(as_stream(stream), ptr(k_pool), ptr(ks_pool), ptr(kb_pool), ptr(kbs_pool), static_cast<const int *>(ptr(pages)),
+                              n, nkv, n_pages);
+}
+
+// Rows of one selection + attention launch pair; longer calls take several.  (The grid's z dimension ends at 65535; the lists
+// of 8192 rows are a few megabytes.)
+static constexpr int SPARSE_ROWS = 8192;
+
+// Workspace of a sparse call: the lists of a launch's rows, their lengths, then the attention's split scratch.
+struct SparseWs { int64_t lists, lens, attn; };
+static int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+static int fill_sparse(AttnArgs &a, SparseWs &w, const char *who, int rows, int nh, int nkv, int kvg, int l_hd, int n_pages, int top_pages,
+                       int max_len) {
+    static const int dummy = 0;
+    REQUIRE(top_pages > 0 && max_len > 0, "%s: bad top_pages/max_len", who);
+    const int64_t pages = std::min<int64_t>(top_pages, ((int64_t)max_len + 127) / 128);
+    int rc = fill_paged(a, who, 0, 0, 0, 0, 0, (uint64_t)(uintptr_t)&dummy, (uint64_t)(uintptr_t)&dummy, 0, 0, 0, rows, nh, nkv, kvg, l_hd,
+                        n_pages, top_pages, (int)std::min<int64_t>(pages * 128, 0x7fffff80), 1.0, ET_F32, ET_F32);
+    if (rc) return rc;
+    a.unit_lists = 1;
+    const int64_t attn = attn_paged_workspace_bytes(a);
+    if (attn < 0) return (int)attn;
+    w.lists = align16((int64_t)rows * nkv * top_pages * 4);
+    w.lens = align16((int64_t)rows * nkv * 4);
+    w.attn = attn;
+    return NOMOS_OK;
+}
+
+NOMOS_EXPORT int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd,
+                                                             int32_t top_pages, int32_t max_len) {
+    const char *who = "nomos_attn_paged_sparse_workspace_bytes";
+    if (rows <= 0) return 0;
+    int64_t most = 0;
+    for (int r : {std::min(rows, SPARSE_ROWS), rows % SPARSE_ROWS}) {   // full launches, and the last one with its own split
+        if (r == 0) continue;
+        AttnArgs a;
+        SparseWs w;
+        int rc = fill_sparse(a, w, who, r, nh, nkv, kvg, l_hd, 1, top_pages, max_len);
+        if (rc) return rc;
+        most = std::max(most, w.lists + w.lens + w.attn);
+    }
+    return most;
+}
+
+NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, uint64_t q, uint64_t k_pool, uint64_t v_pool, uint64_t ks_pool,
+                                                uint64_t vs_pool, uint64_t kb_pool, uint64_t kbs_pool, uint64_t block_table,
+                                                uint64_t row_seq, uint64_t row_pos, uint64_t out, uint64_t sel_pages, uint64_t workspace,
+                                                int64_t ws_bytes, int32_t rows, int32_t batch, int32_t nh, int32_t nkv, int32_t kvg,
+                                                int32_t l_hd, int32_t n_pages, int32_t max_pages, int32_t max_len, int32_t top_pages,
+                                                int32_t sink_pages, int32_t local_pages, double softmax_scale, int32_t q_type,
+                                                int32_t out_type) {
+    const char *who = "nomos_attn_paged_sparse_i8";
+    if (rows <= 0 || batch <= 0 || nh <= 0 || max_len <= 0) return NOMOS_OK;
+    REQUIRE(q && k_pool && v_pool && ks_pool && vs_pool && kb_pool && kbs_pool && block_table && row_seq && row_pos && out && workspace,
+            "%s: null pointer", who);
+    int rc = check_page_pool(who, nkv, l_hd, n_pages);
+    if (rc) return rc;
+    REQUIRE((q_type == ET_F32 || q_type == ET_BF16) && (out_type == ET_F32 || out_type == ET_BF16), "%s: element type", who);
+    REQUIRE(aligned(k_pool, 16) && aligned(v_pool, 16) && aligned(ks_pool, 16) && aligned(vs_pool, 16) && aligned(kb_pool, 16) &&
+                aligned(kbs_pool, 4) && aligned(q, 4) && aligned(out, 4) && aligned(block_table, 4) && aligned(row_seq, 4) &&
+                aligned(row_pos, 4) && aligned(sel_pages, 4) && aligned(workspace, 16), "%s: misaligned buffer", who);
+    REQUIRE(max_pages > 0 && (int64_t)max_pages * 128 >= max_len, "%s: max_len %d exceeds max_pages %d x 128", who, max_len, max_pages);
+    REQUIRE(sink_pages >= 0 && local_pages >= 1 && (int64_t)sink_pages + local_pages <= top_pages,
+            "%s: %d first and %d last pages (at least the row's own) of %d selected", who, sink_pages, local_pages, top_pages);
+    REQUIRE(softmax_scale > 0.0 && softmax_scale <= 3.4e38, "%s: the bounds order pages for a positive softmax scale only", who);
+    if (((int64_t)max_len + 127) / 128 > SELECT_MAX_PAGES && ((int64_t)max_len + 127) / 128 > top_pages) {
+        set_error("%s: selection from more than %d pages", who, SELECT_MAX_PAGES);
+        return NOMOS_EUNSUPPORTED;
+    }
+    const size_t qs = q_type == ET_BF16 ? 2 : 4, os = out_type == ET_BF16 ? 2 : 4;
+    for (int r0 = 0; r0 < rows; r0 += SPARSE_ROWS) {
+        const int nr = std::min(SPARSE_ROWS, rows - r0);
+        AttnArgs a;
+        SparseWs w;
+        rc = fill_sparse(a, w, who, nr, nh, nkv, kvg, l_hd, n_pages, top_pages, max_len);
+        if (rc) return rc;
+        if (w.lists + w.lens + w.attn > ws_bytes) {
+            set_error("%s: workspace too small: need %ld bytes, have %ld", who, (long)(w.lists + w.lens + w.attn), (long)ws_bytes);
+            return NOMOS_ECAPACITY;
+        }
+        PagedSelect s;
+        s.q = ptr(q + (uint64_t)r0 * nh * l_hd * qs); s.kb_pool = ptr(kb_pool); s.kbs_pool = ptr(kbs_pool);
+        s.block_table = static_cast<const int *>(ptr(block_table));
+        s.row_seq = static_cast<const int *>(ptr(row_seq)) + r0; s.row_pos = static_cast<const int *>(ptr(row_pos)) + r0;
+        s.lists = static_cast<int *>(ptr(workspace)); s.lens = static_cast<int *>(ptr(workspace + w.lists));
+        s.sel = sel_pages ? static_cast<int *>(ptr(sel_pages)) + (size_t)r0 * nkv * top_pages : nullptr;
+        s.q_bf16 = q_type == ET_BF16; s.rows = nr; s.batch = batch; s.nh = nh; s.nkv = nkv; s.kvg = kvg; s.n_pages = n_pages;
+        s.max_pages = max_pages; s.max_len = max_len; s.top = top_pages; s.sink = sink_pages; s.local = local_pages;
+        a.q = s.q; a.k_cache = ptr(k_pool); a.v_cache = ptr(v_pool); a.k_scales = ptr(ks_pool); a.v_scales = ptr(vs_pool);
+        a.out = ptr(out + (uint64_t)r0 * nh * l_hd * os);
+        a.block_table = s.lists; a.seq_lens = s.lens;
+        a.workspace = ptr(workspace + w.lists + w.lens); a.ws_bytes = w.attn;
+        a.softmax_scale = (float)softmax_scale; a.q_type = q_type; a.out_type = out_type;
+        rc = launch_paged_select(as_stream(stream), s);
+        if (rc) return rc;
+        rc = launch_attn_paged(as_stream(stream), a);
+        if (rc) return rc;
+    }
+    return NOMOS_OK;
+}
+
+NOMOS_EXPORT int32_t nomos_attn_spec_verify(void *stream, uint64_t target_probs, uint64_t draft_probs, uint64_t draft_tokens, uint64_t n_draft,
+                                            uint64_t u_accept, uint64_t u_sample, uint64_t seq_lens, uint64_t seq_lens_out,
+                                            uint64_t n_accepted, uint64_t out_tokens, int32_t batch, int32_t max_draft, int32_t vocab,
+                                            int64_t p_stride, int64_t q_stride) {
+    const char *who = "nomos_attn_spec_verify";
+    if (batch <= 0) return NOMOS_OK;
+    REQUIRE(max_draft >= 0 && vocab > 0, "%s: bad max_draft/vocab", who);
+    REQUIRE(target_probs && u_sample && n_accepted && out_tokens && (max_draft == 0 || (draft_tokens && u_accept)), "%s: null pointer", who);
+    REQUIRE((seq_lens != 0) == (seq_lens_out != 0), "%s: lengths need an input and an output", who);
+    REQUIRE(p_stride >= vocab && (!draft_probs || q_stride >= vocab), "%s: rows of %d probabilities, fewer apart", who, vocab);
+    for (uint64_t x : {target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens})
+        REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);
+    const auto f = [](uint64_t a) { return static_cast<const float *>(ptr(a)); };
+    const auto i = [](uint64_t a) { return static_cast<int *>(ptr(a)); };
+    return launch_spec_verify(as_stream(stream), f(target_probs), max_draft > 0 ? f(draft_probs) : nullptr, i(draft_tokens), i(n_draft),
+                              f(u_accept), f(u_sample), i(seq_lens), i(seq_lens_out), i(n_accepted), i(out_tokens), batch, max_draft, vocab,
+                              p_stride, q_stride);
 }
 
 NOMOS_EXPORT int32_t nomos_attn_merge_partials(void *stream, uint64_t partials, int32_t G, int32_t rows, int32_t l_hd,

@@ -617,6 +617,7 @@ static int launch_tc5_inst(cudaStream_t st, const AttnArgs &a, bool query_ws, lo
     const long part_bytes = (((long)pl.splits * pl.grows * (a.l_hd + 2) * 4) + 15) / 16 * 16;
     const bool in_kernel_merge = pl.splits > 1 || a.peer_world > 1;
     const long need = in_kernel_merge ? part_bytes + units * 16 : 0;
+    if (query_ws && a.unit_lists) { *ws_needed = need; return NOMOS_OK; }      // many rows, mostly one split each
     if (query_ws) { *ws_needed = part_bytes + units * 16; return NOMOS_OK; }   // also enough for a sequence-sharded call, which merges in the kernel even with one split
     if (need > a.ws_bytes || (need > 0 && a.workspace == nullptr)) {
         set_error("attention workspace too small: need %ld bytes, have %ld", need, a.ws_bytes);
@@ -661,6 +662,7 @@ static int launch_tc5_inst(cudaStream_t st, const AttnArgs &a, bool query_ws, lo
     // 125.7 -> 124.9, 1107 MB: 166.5 -> 167.0; the mma.sync kernel gains 3 to 4 % at all three)
     p.kv_read_once = (pl.row_groups == 1 && (long)a.batch * a.nkv * a.klen * 2 * a.cache_hd < (1024l << 20)) ? 1 : 0;
     p.block_table = a.block_table; p.seq_lens = a.seq_lens; p.max_pages = a.max_pages;
+    p.unit_lists = a.unit_lists;
     p.q_type = a.q_type; p.out_type = a.out_type;
     p.S = a.S; p.nh = a.nh; p.nkv = a.nkv; p.kvg = a.kvg; p.cache_hd = a.cache_hd; p.cache_cap = a.cache_cap;
     p.win_start = a.win_start; p.klen = a.klen; p.window = a.window;

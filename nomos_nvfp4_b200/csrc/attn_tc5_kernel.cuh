@@ -389,12 +389,20 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
         fused::pdl_launch_dependents();
     }
     if (paged) {
-        const int len = p.seq_lens[b];
+        // a list of pages per sequence, or (unit_lists) per query row and KV head
+        const size_t tb = p.unit_lists ? (size_t)b * p.nkv + kvh : (size_t)b;
+        const int len = p.seq_lens[tb];
+        if (p.unit_lists && len <= 0) {                  // a row that is skipped: its output stays as it is
+            tc_fence_before();
+            __syncthreads();
+            if (warp == NSW) tmem_dealloc(tmem_base, C::TMEM_COLS);
+            return;
+        }
         wg.klen = len; wg.ring0 = 0; wg.a0 = 0; wg.len_a = len;
         wg.n_a = (len + KT - 1) / KT;
         tile_end = min(wg.n_a, tile_begin + p.tiles_per_split);
         my_n = max(0, tile_end - tile_begin);
-        for (int i = threadIdx.x; i < my_n; i += NTHREADS) page_ids[i] = p.block_table[(size_t)b * p.max_pages + tile_begin + i];
+        for (int i = threadIdx.x; i < my_n; i += NTHREADS) page_ids[i] = p.block_table[tb * p.max_pages + tile_begin + i];
         __syncthreads();
     }
 

@@ -16,6 +16,29 @@ int launch_append_i8(cudaStream_t st, const void *src_k, const void *src_v, void
 int launch_append_paged_i8(cudaStream_t st, const void *src_k, const void *src_v, void *k_pool, void *v_pool, void *ks_pool,
                            void *vs_pool, const int *block_table, const int *positions, int batch, int nkv, int l_hd, int l_kvd,
                            int max_pages);
+// ---- paged_plan.cu
+constexpr int PLAN_MAX_BATCH = 8192;     // requests of one call: their prefix sums live in shared memory
+int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, const int *held, int *free_pages, const int *free_count,
+                      int *block_table, int *held_out, int *free_count_out, int *granted, int *row_start, int *slot_map, int *row_seq,
+                      int *row_pos, int batch, int max_pages, int n_pages, int max_rows);
+// ---- paged_rows.cu (kb_pool nullptr: no page bounds)
+int launch_append_slots_i8(cudaStream_t st, const void *src_k, const void *src_v, void *k_pool, void *v_pool, void *ks_pool, void *vs_pool,
+                           void *kb_pool, void *kbs_pool, const int *slot_map, int n_rows, int nkv, int l_kvd, int n_pages, int src_bf16);
+int launch_page_bounds(cudaStream_t st, const void *k_pool, const void *ks_pool, void *kb_pool, void *kbs_pool, const int *pages, int n,
+                       int nkv, int n_pages);
+// ---- paged_select.cu
+constexpr int SELECT_MAX_PAGES = 49152;  // pages of one sequence: their scores live in shared memory
+struct PagedSelect {
+    const void *q, *kb_pool, *kbs_pool;
+    const int *block_table, *row_seq, *row_pos;
+    int *lists, *lens, *sel;
+    int q_bf16, rows, batch, nh, nkv, kvg, n_pages, max_pages, max_len, top, sink, local;
+};
+int launch_paged_select(cudaStream_t st, const PagedSelect &s);
+// ---- spec_verify.cu
+int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const int *tokens, const int *n_draft, const float *u_accept,
+                       const float *u_sample, const int *lens, int *lens_out, int *n_accepted, int *out_tokens, int batch, int max_draft,
+                       int vocab, long p_stride, long q_stride);
 int launch_append_i4(cudaStream_t st, const void *src_k, const void *src_v, void *dst_k, void *dst_v, void *k_scales,
                      void *v_scales, void *k_q8, void *v_q8, void *k_q8_scales, void *v_q8_scales, int n_s, int nkv,
                      int l_hd, int l_kvd, int cache_cap, int cache_hd, int base_pos, int q8_pitch, int scale_blocks);
@@ -59,6 +82,8 @@ struct AttnArgs {
     const int *block_table;
     const int *seq_lens;
     int max_pages, n_pages;
+    int unit_lists;         // 1: block_table [batch][nkv][max_pages] and seq_lens [batch][nkv] (pages listed per query row and
+                            // KV head; batch counts query rows); a unit of length 0 is skipped, its output left as it is
     // sequence-sharded decode across GPUs (peer_world > 1, see nomos_attn_seq_sharded): every rank's mailbox as mapped
     // in this process, this rank's index, the step number and the wait limit
     void *peer_box[8];

@@ -1,0 +1,229 @@
+// Block tables and slot maps of a serving step, from request lengths (sm_100a).  Integer work only:
+//   end_b   = sum of max(n_new, 0) up to and including request b              (rows of the step)
+//   need_b  = pages request b lacks for len_b + n_b keys, 0 where it cannot be served
+//   upto_b  = sum of need up to and including b: granted while upto_b fits the free pages (finished requests' included)
+// A few thousand requests are three prefix sums; what costs is the latency of one launch and the 12 bytes written per row.
+// So every CTA of one thread-block cluster works the sums out for itself in shared memory (no global scratch, no second
+// launch) and the CTAs share the rows.  held_out may be held itself and free_count_out free_count: the cluster meets once
+// between the last read of the inputs and the first write.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "launch.h"
+
+namespace nomos {
+
+constexpr int PLAN_PAGE = 128;           // keys per page
+constexpr int PLAN_THREADS = 1024;
+
+struct PlanParams {
+    const int *seq_lens, *n_new, *held;
+    int *free_pages;
+    const int *free_count;
+    int *block_table, *held_out, *free_count_out, *granted, *row_start, *slot_map, *row_seq, *row_pos;
+    int batch, max_pages, n_pages, max_rows;
+    int vec;                             // the three row arrays start on 16-byte boundaries
+};
+
+struct Pair64 { long long a, b; };
+
+// Inclusive prefix sums of two numbers over the block; tot = the block's sums.  `scratch`: 33 entries.
+__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64 *scratch, Pair64 &tot) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long a = __shfl_up_sync(0xffffffffu, v.a, o), b = __shfl_up_sync(0xffffffffu, v.b, o);
+        if (lane >= o) { v.a += a; v.b += b; }
+    }
+    __syncthreads();                     // the scratch may still be read from the previous scan
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        Pair64 w = lane < nwarp ? scratch[lane] : Pair64{0, 0};
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long a = __shfl_up_sync(0xffffffffu, w.a, o), b = __shfl_up_sync(0xffffffffu, w.b, o);
+            if (lane >= o) { w.a += a; w.b += b; }
+        }
+        scratch[lane] = w;
+    }
+    __syncthreads();
+    if (warp > 0) { v.a += scratch[warp - 1].a; v.b += scratch[warp - 1].b; }
+    tot = scratch[31];
+    return v;
+}
+
+// First index i with v[i] > x, v ascending, x < v[n - 1].
+__device__ __forceinline__ int first_above(const int *v, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] > x) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_constant__ PlanParams p) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    extern __shared__ int plan_sm[];
+    const int B = p.batch;
+    int *s_end = plan_sm;                // rows up to and including the request, at most max_rows
+    int *s_len = s_end + B;              // keys cached so far
+    int *s_held = s_len + B;             // pages held; -1 - pages: not served in this step
+    int *s_upto = s_held + B;            // pages needed up to and including the request
+    int *s_rel = s_upto + B;             // pages released up to and including the request
+    __shared__ Pair64 scratch[33];
+    __shared__ int s_taken;
+
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    if (threadIdx.x == 0) s_taken = 0;
+    const int F = max(0, min(p.free_count[0], p.n_pages));
+    const int per = (B + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per, b1 = min(B, b0 + per);
+
+    // rows
+    long long rows = 0;
+    for (int b = b0; b < b1; ++b) rows += max(p.n_new[b], 0);
+    Pair64 tot;
+    const Pair64 re = block_scan(Pair64{rows, 0}, scratch, tot);
+    const int total_rows = (int)min(tot.a, (long long)p.max_rows);
+    long long end = re.a - rows, need_sum = 0, rel_sum = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int n = p.n_new[b], len = max(p.seq_lens[b], 0), held = max(0, min(p.held[b], p.max_pages));
+        end += max(n, 0);
+        const long long keys = (long long)len + n;
+        const bool fits = n > 0 && end <= p.max_rows && keys <= (long long)p.max_pages * PLAN_PAGE;
+        const int need = fits ? max(0, (int)((keys + PLAN_PAGE - 1) / PLAN_PAGE) - held) : 0;
+        const int rel = n < 0 ? held : 0;
+        s_end[b] = (int)min(end, (long long)p.max_rows);
+        s_len[b] = len;
+        s_held[b] = fits ? held : -1 - held;
+        s_upto[b] = need;
+        s_rel[b] = rel;
+        need_sum += need;
+        rel_sum += rel;
+    }
+    // pages: a request's need and release become prefix sums (saturated: a sum beyond the pool is never granted)
+    const Pair64 pr = block_scan(Pair64{need_sum, rel_sum}, scratch, tot);
+    const int R = (int)min(tot.b, (long long)p.n_pages);
+    const long long avail = (long long)F + R;
+    long long upto = pr.a - need_sum, rel = pr.b - rel_sum;
+    int taken = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int need = s_upto[b];
+        upto += need;
+        rel += s_rel[b];
+        if (s_held[b] >= 0 && need > 0) {
+            if (upto <= avail) taken = (int)upto;                   // upto only grows: what is granted is a prefix
+            else s_held[b] = -1 - s_held[b];
+        }
+        s_upto[b] = (int)min(upto, 0x7fffffffll);
+        s_rel[b] = (int)min(rel, 0x7fffffffll);
+    }
+    if (taken > 0) atomicMax(&s_taken, taken);
+    // everything that may be overwritten in place has been read: the cluster's CTAs may write from here on
+    if (gridDim.x > 1) cluster.sync();
+    else __syncthreads();
+    const int T = s_taken;
+
+    // page at index i of the stack of free pages, the finished requests' pages on top of it
+    auto released = [&](int e) {
+        const int b = first_above(s_rel, B, e);
+        const int before = b > 0 ? s_rel[b - 1] : 0;
+        return p.block_table[(size_t)b * p.max_pages + (e - before)];
+    };
+    auto stack = [&](int i) { return i < F ? p.free_pages[i] : released(i - F); };
+    auto need_before = [&](int b) { return b > 0 ? s_upto[b - 1] : 0; };
+    const int top = (int)avail - 1;
+    auto page_of = [&](int b, int j) {
+        const int held = s_held[b];
+        return j < held ? p.block_table[(size_t)b * p.max_pages + j] : stack(top - need_before(b) - (j - held));
+    };
+    const int tid = blockIdx.x * blockDim.x + threadIdx.x, nthreads = gridDim.x * blockDim.x;
+
+    // rows: four consecutive ones per thread, one search for the four
+    for (long long r0 = 4ll * tid; r0 < p.max_rows; r0 += 4ll * nthreads) {
+        int slot[4], seq[4], pos[4];
+        int b = r0 < total_rows ? first_above(s_end, B, (int)r0) : B, last_b = -1, last_j = -1, page = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = (int)min(r0 + k, (long long)p.max_rows - 1);
+            while (b < B && s_end[b] <= r) ++b;
+            slot[k] = seq[k] = pos[k] = -1;
+            if (r < total_rows && b < B && s_held[b] >= 0) {
+                const int at = s_len[b] + (r - (b > 0 ? s_end[b - 1] : 0)), j = at / PLAN_PAGE;
+                if (b != last_b || j != last_j) { page = page_of(b, j); last_b = b; last_j = j; }
+                slot[k] = (int)((unsigned)page * PLAN_PAGE + (unsigned)(at % PLAN_PAGE));
+                seq[k] = b;
+                pos[k] = at;
+            }
+        }
+        if (p.vec && r0 + 4 <= p.max_rows) {
+            *reinterpret_cast<int4 *>(p.slot_map + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            *reinterpret_cast<int4 *>(p.row_seq + r0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+            *reinterpret_cast<int4 *>(p.row_pos + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (r0 + k < p.max_rows) {
+                    p.slot_map[r0 + k] = slot[k];
+                    p.row_seq[r0 + k] = seq[k];
+                    p.row_pos[r0 + k] = pos[k];
+                }
+        }
+    }
+    // the new pages' table entries, and the released pages back onto the stack.  (No CTA reads a table entry or a stack
+    // entry that another one writes: new entries lie behind the held ones, pushes at or above F.)
+    for (int e = tid; e < T; e += nthreads) {
+        const int b = first_above(s_upto, B, e), i = e - need_before(b);
+        p.block_table[(size_t)b * p.max_pages + s_held[b] + i] = stack(top - e);
+    }
+    for (int e = tid; e < R; e += nthreads)
+        if (F + e < p.n_pages) p.free_pages[F + e] = released(e);
+    if (blockIdx.x == 0) {
+        for (int b = threadIdx.x; b < B; b += blockDim.x) {
+            const int h = s_held[b], n_b = s_end[b] - (b > 0 ? s_end[b - 1] : 0);
+            const int need = s_upto[b] - need_before(b), rel_b = s_rel[b] - (b > 0 ? s_rel[b - 1] : 0);
+            p.granted[b] = h >= 0 ? n_b : 0;
+            p.held_out[b] = h >= 0 ? h + need : -1 - h - rel_b;     // a finished request releases what it held
+            p.row_start[b + 1] = s_end[b];
+        }
+        if (threadIdx.x == 0) {
+            p.row_start[0] = 0;
+            p.free_count_out[0] = (int)min(avail - T, (long long)p.n_pages);
+        }
+    }
+}
+
+int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, const int *held, int *free_pages, const int *free_count,
+                      int *block_table, int *held_out, int *free_count_out, int *granted, int *row_start, int *slot_map, int *row_seq,
+                      int *row_pos, int batch, int max_pages, int n_pages, int max_rows) {
+    PlanParams p{seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start, slot_map,
+                 row_seq, row_pos, batch, max_pages, n_pages, max_rows, 0};
+    p.vec = ((reinterpret_cast<uintptr_t>(slot_map) | reinterpret_cast<uintptr_t>(row_seq) | reinterpret_cast<uintptr_t>(row_pos)) & 15) == 0;
+    const size_t smem = (size_t)batch * 5 * sizeof(int);
+    cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_MAX_BATCH * 5 * (int)sizeof(int)) : cudaSuccess;
+    if (e != cudaSuccess) { set_error("nomos_kv_paged_plan: shared memory: %s", cudaGetErrorString(e)); return NOMOS_ECUDA; }
+    // one CTA while its threads cover the rows in one round, else a cluster of eight
+    const int ctas = max_rows <= 4 * PLAN_THREADS ? 1 : 8;
+    const int most = std::max(batch, (max_rows + 3) / 4);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(ctas > 1 ? PLAN_THREADS : std::min(PLAN_THREADS, (most + 31) / 32 * 32));
+    cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, paged_plan_kernel, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) { set_error("nomos_kv_paged_plan: %s", cudaGetErrorString(e)); return NOMOS_ECUDA; }
+    return NOMOS_OK;
+}
+
+}  // namespace nomos

@@ -319,6 +319,58 @@ def kv_paged_append_quant_i8(stream, src_k, src_v, k_pool, v_pool, ks_pool, vs_p
         _addr(block_table), _addr(positions), batch, nkv, l_hd, l_kvd, max_pages))
 
 
+def kv_paged_plan(stream, seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start,
+                  slot_map, row_seq, row_pos, *, batch, max_pages, n_pages, max_rows):
+    """Block tables and slot maps of a step from request lengths, all int32 on the GPU; see include/nomos_attn.h.
+    ``n_new`` < 0 hands a finished request's pages back; ``granted`` tells which requests got their pages."""
+    _check(_lib.lib().nomos_kv_paged_plan(
+        _stream(stream), _addr(seq_lens), _addr(n_new), _addr(held), _addr(free_pages), _addr(free_count), _addr(block_table), _addr(held_out),
+        _addr(free_count_out), _addr(granted), _addr(row_start), _addr(slot_map), _addr(row_seq), _addr(row_pos), batch, max_pages, n_pages,
+        max_rows))
+
+
+def kv_paged_append_rows_i8(stream, src_k, src_v, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, slot_map, *, n_rows, nkv, l_hd, l_kvd,
+                            n_pages, src_type=F32):
+    """Quantising append of any number of rows by slot map; with ``kb_pool`` / ``kbs_pool`` (else ``None``) also the bounds of
+    every page whose last row is among them."""
+    _check(_lib.lib().nomos_kv_paged_append_rows_i8(
+        _stream(stream), _addr(src_k), _addr(src_v), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool),
+        _addr(kbs_pool), _addr(slot_map), n_rows, nkv, l_hd, l_kvd, n_pages, src_type))
+
+
+def kv_paged_page_bounds_i8(stream, k_pool, ks_pool, kb_pool, kbs_pool, pages, *, n, nkv, l_hd, n_pages):
+    """Page bounds of the ``n`` listed pages (int32; entries outside the pool are skipped), for pages filled another way."""
+    _check(_lib.lib().nomos_kv_paged_page_bounds_i8(_stream(stream), _addr(k_pool), _addr(ks_pool), _addr(kb_pool), _addr(kbs_pool), _addr(pages),
+                                                    n, nkv, l_hd, n_pages))
+
+
+def attn_paged_sparse_workspace_bytes(*, rows, nh, nkv, kvg, l_hd, top_pages, max_len) -> int:
+    n = _lib.lib().nomos_attn_paged_sparse_workspace_bytes(rows, nh, nkv, kvg, l_hd, top_pages, max_len)
+    if n < 0:
+        _check(int(n))
+    return int(n)
+
+
+def attn_paged_sparse_i8(stream, q, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, block_table, row_seq, row_pos, out, sel_pages, workspace,
+                         ws_bytes, *, rows, batch, nh, nkv, kvg, l_hd, n_pages, max_pages, max_len, top_pages, sink_pages=1, local_pages=1,
+                         softmax_scale=1.0, q_type=F32, out_type=F32):
+    """Attention of ``rows`` query rows (decode, verify and prompt rows alike: sequence ``row_seq[r]``, position ``row_pos[r]``)
+    over at most ``top_pages`` pages each, selected per row and KV head by a bound on the logits; see include/nomos_attn.h."""
+    _check(_lib.lib().nomos_attn_paged_sparse_i8(
+        _stream(stream), _addr(q), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool), _addr(kbs_pool),
+        _addr(block_table), _addr(row_seq), _addr(row_pos), _addr(out), _addr(sel_pages), _addr(workspace), int(ws_bytes), rows, batch, nh, nkv,
+        kvg, l_hd, n_pages, max_pages, max_len, top_pages, sink_pages, local_pages, float(softmax_scale), q_type, out_type))
+
+
+def spec_verify(stream, target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens, *,
+                batch, max_draft, vocab, p_stride, q_stride):
+    """Speculative verification from given random numbers: accepted drafts, and the next token from the residual (or, all
+    accepted, from the target's last row); see include/nomos_attn.h.  ``draft_probs``, ``n_draft``, ``seq_lens`` may be ``None``."""
+    _check(_lib.lib().nomos_attn_spec_verify(
+        _stream(stream), _addr(target_probs), _addr(draft_probs), _addr(draft_tokens), _addr(n_draft), _addr(u_accept), _addr(u_sample),
+        _addr(seq_lens), _addr(seq_lens_out), _addr(n_accepted), _addr(out_tokens), batch, max_draft, vocab, p_stride, q_stride))
+
+
 class KvRing:
     """One layer's ring bookkeeping (``nomos_kv_ring_*``): lengths, window arithmetic, staged rows,
     roll-back.  ``window`` = 0 is a linear cache.  A ring that serves batches of ``max_rows`` rows needs
