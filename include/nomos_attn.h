@@ -440,7 +440,7 @@ int32_t nomos_kv_paged_append_quant_i8(void *stream, uint64_t src_k, uint64_t sr
  *   nomos_attn_paged_sparse_i8     attention of every row over the pages its bounds select (top_pages >= the sequence's
  *                                  pages: over all of them)
  *   nomos_attn_spec_verify         drafted tokens against the target's probabilities, lengths advanced
- * Integer arrays are int32.
+ * Integer arrays are int32.  Argument blocks: all fields 8 bytes wide, struct_bytes = sizeof the block.
  *
  * Block tables and slot maps.  Request b has seq_lens[b] keys cached, brings n_new[b] rows and holds held[b] pages, the first
  * held[b] entries of its row of block_table [batch][max_pages].  free_pages [n_pages] is a stack of free_count[0] page numbers.
@@ -457,19 +457,25 @@ int32_t nomos_kv_paged_append_quant_i8(void *stream, uint64_t src_k, uint64_t sr
  * their own a plan can be dropped: the entries it wrote lie behind what held and free_count count.  seq_lens is not written:
  * add what was kept (nomos_attn_spec_verify does), so rows rejected there are planned again, into the pages already held.
  * At most 8192 requests. */
-int32_t nomos_kv_paged_plan(void *stream, uint64_t seq_lens, uint64_t n_new, uint64_t held, uint64_t free_pages, uint64_t free_count,
-                            uint64_t block_table, uint64_t held_out, uint64_t free_count_out, uint64_t granted, uint64_t row_start,
-                            uint64_t slot_map, uint64_t row_seq, uint64_t row_pos, int32_t batch, int32_t max_pages, int32_t n_pages,
-                            int32_t max_rows);
+typedef struct nomos_kv_plan {
+    uint64_t struct_bytes;
+    uint64_t seq_lens, n_new, held, free_pages, free_count, block_table;
+    uint64_t held_out, free_count_out, granted, row_start, slot_map, row_seq, row_pos;
+    int64_t batch, max_pages, n_pages, max_rows;
+} nomos_kv_plan_t;
+int32_t nomos_kv_paged_plan(void *stream, const nomos_kv_plan_t *args);
 /* Quantising append of n_rows rows (src [n_rows][nkv][l_hd] of src_type, row stride l_kvd elements) into slots slot_map[r] of
  * the pools, with the row codec of nomos_kv_append_quant_i8.  Slots outside the pool (-1: padding) are skipped; a slot may
  * occur once.  With kb_pool and kbs_pool (else both 0) the bounds of each page whose row 127 is among the slots are computed
  * once all rows are in: kb_pool [n_pages][nkv][2][128] int8 (16-byte aligned), kbs_pool [n_pages][nkv] fp32.  With v the page's
  * dequantised keys, per channel the largest and the smallest, divided by t = (largest magnitude) / 127 and rounded up and
  * down: t * kb[0] >= v >= t * kb[1] up to one rounding.  A page with a row scale that is not finite gets t = +inf, codes 0. */
-int32_t nomos_kv_paged_append_rows_i8(void *stream, uint64_t src_k, uint64_t src_v, uint64_t k_pool, uint64_t v_pool, uint64_t ks_pool,
-                                      uint64_t vs_pool, uint64_t kb_pool, uint64_t kbs_pool, uint64_t slot_map, int32_t n_rows,
-                                      int32_t nkv, int32_t l_hd, int32_t l_kvd, int32_t n_pages, int32_t src_type);
+typedef struct nomos_kv_rows {
+    uint64_t struct_bytes;
+    uint64_t src_k, src_v, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, slot_map;
+    int64_t n_rows, nkv, l_hd, l_kvd, n_pages, src_type;
+} nomos_kv_rows_t;
+int32_t nomos_kv_paged_append_rows_i8(void *stream, const nomos_kv_rows_t *args);
 /* The same bounds for n listed pages (entries outside the pool are skipped): for pages filled by
  * nomos_kv_paged_append_quant_i8 or copied in. */
 int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks_pool, uint64_t kb_pool, uint64_t kbs_pool, uint64_t pages,
@@ -489,12 +495,15 @@ int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks
  * The workspace (16-byte aligned) must not be shared by calls that can overlap on the GPU. */
 int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t top_pages,
                                                 int32_t max_len);
-int32_t nomos_attn_paged_sparse_i8(void *stream, uint64_t q, uint64_t k_pool, uint64_t v_pool, uint64_t ks_pool, uint64_t vs_pool,
-                                   uint64_t kb_pool, uint64_t kbs_pool, uint64_t block_table, uint64_t row_seq, uint64_t row_pos,
-                                   uint64_t out, uint64_t sel_pages, uint64_t workspace, int64_t ws_bytes, int32_t rows, int32_t batch,
-                                   int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t n_pages, int32_t max_pages,
-                                   int32_t max_len, int32_t top_pages, int32_t sink_pages, int32_t local_pages, double softmax_scale,
-                                   int32_t q_type, int32_t out_type);
+typedef struct nomos_attn_sparse {
+    uint64_t struct_bytes;
+    uint64_t q, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, block_table, row_seq, row_pos, out, sel_pages, workspace;
+    int64_t ws_bytes;
+    int64_t rows, batch, nh, nkv, kvg, l_hd, n_pages, max_pages, max_len, top_pages, sink_pages, local_pages;
+    double softmax_scale;
+    int64_t q_type, out_type;
+} nomos_attn_sparse_t;
+int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_sparse_t *args);
 /* Verification of drafted tokens from given random numbers.  Sequence b drafted n_draft[b] tokens (0 pointer: max_draft each;
  * negative: the sequence is idle and nothing of it is written; more than max_draft count as max_draft).  target_probs
  * [batch][max_draft + 1][p_stride], draft_probs [batch][max_draft][q_stride] fp32 rows of `vocab` probabilities in [0, 1]
@@ -506,9 +515,12 @@ int32_t nomos_attn_paged_sparse_i8(void *stream, uint64_t q, uint64_t k_pool, ui
  * zero.  Whole-number sums make it independent of how the row is split.
  * seq_lens_out[b] = seq_lens[b] + a + 1, the keys that stay cached once the last sampled token's row and the accepted drafts'
  * rows are (seq_lens may be seq_lens_out; both 0: no lengths). */
-int32_t nomos_attn_spec_verify(void *stream, uint64_t target_probs, uint64_t draft_probs, uint64_t draft_tokens, uint64_t n_draft,
-                               uint64_t u_accept, uint64_t u_sample, uint64_t seq_lens, uint64_t seq_lens_out, uint64_t n_accepted,
-                               uint64_t out_tokens, int32_t batch, int32_t max_draft, int32_t vocab, int64_t p_stride, int64_t q_stride);
+typedef struct nomos_attn_verify {
+    uint64_t struct_bytes;
+    uint64_t target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens;
+    int64_t batch, max_draft, vocab, p_stride, q_stride;
+} nomos_attn_verify_t;
+int32_t nomos_attn_spec_verify(void *stream, const nomos_attn_verify_t *args);
 
 /* ------------------------------------------------------------------------- *
  *  Sequence-sharded decode across the GPUs of one node (no counterpart in the reference, which runs on   *

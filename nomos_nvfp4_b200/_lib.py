@@ -7,6 +7,7 @@ The idiom follows the reference's own Python binding (pyhost/host.py:108-144).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import os
@@ -53,6 +54,43 @@ class KvStep(C.Structure):
     _fields_ = [("base_pos", i64), ("n_new", i64), ("win_start", i64), ("klen", i64), ("window", i64)]
 
 
+class KvPlan(C.Structure):
+    """Mirror of ``nomos_kv_plan_t``."""
+    _fields_ = [("struct_bytes", u64), ("seq_lens", u64), ("n_new", u64), ("held", u64), ("free_pages", u64), ("free_count", u64),
+                ("block_table", u64), ("held_out", u64), ("free_count_out", u64), ("granted", u64), ("row_start", u64), ("slot_map", u64),
+                ("row_seq", u64), ("row_pos", u64), ("batch", i64), ("max_pages", i64), ("n_pages", i64), ("max_rows", i64)]
+
+
+class KvRows(C.Structure):
+    """Mirror of ``nomos_kv_rows_t``."""
+    _fields_ = [("struct_bytes", u64), ("src_k", u64), ("src_v", u64), ("k_pool", u64), ("v_pool", u64), ("ks_pool", u64), ("vs_pool", u64),
+                ("kb_pool", u64), ("kbs_pool", u64), ("slot_map", u64), ("n_rows", i64), ("nkv", i64), ("l_hd", i64), ("l_kvd", i64),
+                ("n_pages", i64), ("src_type", i64)]
+
+
+class AttnSparse(C.Structure):
+    """Mirror of ``nomos_attn_sparse_t``."""
+    _fields_ = [("struct_bytes", u64), ("q", u64), ("k_pool", u64), ("v_pool", u64), ("ks_pool", u64), ("vs_pool", u64), ("kb_pool", u64),
+                ("kbs_pool", u64), ("block_table", u64), ("row_seq", u64), ("row_pos", u64), ("out", u64), ("sel_pages", u64),
+                ("workspace", u64), ("ws_bytes", i64), ("rows", i64), ("batch", i64), ("nh", i64), ("nkv", i64), ("kvg", i64), ("l_hd", i64),
+                ("n_pages", i64), ("max_pages", i64), ("max_len", i64), ("top_pages", i64), ("sink_pages", i64), ("local_pages", i64),
+                ("softmax_scale", C.c_double), ("q_type", i64), ("out_type", i64)]
+
+
+class AttnVerify(C.Structure):
+    """Mirror of ``nomos_attn_verify_t``."""
+    _fields_ = [("struct_bytes", u64), ("target_probs", u64), ("draft_probs", u64), ("draft_tokens", u64), ("n_draft", u64), ("u_accept", u64),
+                ("u_sample", u64), ("seq_lens", u64), ("seq_lens_out", u64), ("n_accepted", u64), ("out_tokens", u64), ("batch", i64),
+                ("max_draft", i64), ("vocab", i64), ("p_stride", i64), ("q_stride", i64)]
+
+
+def packer(block) -> struct.Struct:
+    """The bytes of an argument block from its values in order: a step's calls are a few microseconds on the GPU, and converting
+    twenty arguments one by one costs as much (10 against 4 us per call on the host)."""
+    code = {u64: "Q", i64: "q", C.c_double: "d"}
+    return struct.Struct("=" + "".join(code[t] for _, t in block._fields_))
+
+
 # name -> (restype, argtypes); must list every symbol include/nomos_attn.h declares.
 PROTOTYPES = {
     "nomos_kv_ring_init": (i32, [C.POINTER(KvRing), i64, i64, i64]),
@@ -66,12 +104,13 @@ PROTOTYPES = {
     "nomos_attn_paged_workspace_bytes": (i64, [i32] * 6),
     "nomos_attn_paged_decode_i8": (i32, [vp] + [u64] * 9 + [i64] + [i32] * 8 + [C.c_double, i32, i32]),
     "nomos_kv_paged_append_quant_i8": (i32, [vp] + [u64] * 8 + [i32] * 5),
-    "nomos_kv_paged_plan": (i32, [vp] + [u64] * 13 + [i32] * 4),
-    "nomos_kv_paged_append_rows_i8": (i32, [vp] + [u64] * 9 + [i32] * 6),
+    # (argument blocks as bytes, see packer)
+    "nomos_kv_paged_plan": (i32, [vp, C.c_char_p]),
+    "nomos_kv_paged_append_rows_i8": (i32, [vp, C.c_char_p]),
     "nomos_kv_paged_page_bounds_i8": (i32, [vp] + [u64] * 5 + [i32] * 4),
     "nomos_attn_paged_sparse_workspace_bytes": (i64, [i32] * 7),
-    "nomos_attn_paged_sparse_i8": (i32, [vp] + [u64] * 13 + [i64] + [i32] * 12 + [C.c_double, i32, i32]),
-    "nomos_attn_spec_verify": (i32, [vp] + [u64] * 10 + [i32] * 3 + [i64] * 2),
+    "nomos_attn_paged_sparse_i8": (i32, [vp, C.c_char_p]),
+    "nomos_attn_spec_verify": (i32, [vp, C.c_char_p]),
     "nomos_attn_fused_host": (i32, [vp, C.POINTER(AttnArgs), u64, u64, C.c_int64, u64, u64, C.c_int64]),
     "nomos_kv_norm_rope_append": (i32, [vp] + [u64] * 11 + [i32] * 8 + [C.c_float, i32, i32]),
     "nomos_kv_quant_i8": (i32, [vp, u64, u64, u64, i32, i32]),

@@ -4,6 +4,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/nomos_attn.h"
 #include "common.cuh"
@@ -665,53 +666,61 @@ NOMOS_EXPORT int32_t nomos_kv_paged_append_quant_i8(void *stream, uint64_t src_k
 
 // ------------------------------------------------------------------- batch serving on paged caches
 
-NOMOS_EXPORT int32_t nomos_kv_paged_plan(void *stream, uint64_t seq_lens, uint64_t n_new, uint64_t held, uint64_t free_pages,
-                                         uint64_t free_count, uint64_t block_table, uint64_t held_out, uint64_t free_count_out,
-                                         uint64_t granted, uint64_t row_start, uint64_t slot_map, uint64_t row_seq, uint64_t row_pos,
-                                         int32_t batch, int32_t max_pages, int32_t n_pages, int32_t max_rows) {
-    const char *who = "nomos_kv_paged_plan";
-    if (batch <= 0) return NOMOS_OK;
-    REQUIRE(seq_lens && n_new && held && free_pages && free_count && block_table && held_out && free_count_out && granted && row_start,
-            "%s: null pointer", who);
-    REQUIRE(max_rows >= 0 && (max_rows == 0 || (slot_map && row_seq && row_pos)), "%s: null pointer or negative max_rows", who);
-    REQUIRE(max_pages > 0 && n_pages > 0, "%s: bad max_pages/n_pages", who);
-    for (uint64_t x : {seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start, slot_map,
-                       row_seq, row_pos})
-        REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);
-    REQUIRE((int64_t)max_pages * 128 < (1l << 31) && (int64_t)n_pages * 128 < (1l << 31), "%s: positions and slots are 32-bit numbers", who);
-    if (batch > PLAN_MAX_BATCH) { set_error("%s: at most %d requests per call", who, PLAN_MAX_BATCH); return NOMOS_EUNSUPPORTED; }
-    const auto in = [](uint64_t a) { return static_cast<const int *>(ptr(a)); };
-    const auto io = [](uint64_t a) { return static_cast<int *>(ptr(a)); };
-    return launch_paged_plan(as_stream(stream), in(seq_lens), in(n_new), in(held), io(free_pages), in(free_count), io(block_table), io(held_out),
-                             io(free_count_out), io(granted), io(row_start), io(slot_map), io(row_seq), io(row_pos), batch, max_pages, n_pages,
-                             max_rows);
+// Argument blocks: every dimension is a 64-bit field that has to fit 32 bits.
+#define REQUIRE_BLOCK(args, T) \
+    REQUIRE((args) != nullptr && (args)->struct_bytes == sizeof(T), "%s: argument block of another version", who)
+static bool fits32(std::initializer_list<int64_t> v) {
+    for (int64_t x : v)
+        if (x != (int32_t)x) return false;
+    return true;
 }
 
-static int check_page_pool(const char *who, int nkv, int l_hd, int n_pages) {
+NOMOS_EXPORT int32_t nomos_kv_paged_plan(void *stream, const nomos_kv_plan_t *a) {
+    const char *who = "nomos_kv_paged_plan";
+    REQUIRE_BLOCK(a, nomos_kv_plan_t);
+    if (a->batch <= 0) return NOMOS_OK;
+    REQUIRE(a->seq_lens && a->n_new && a->held && a->free_pages && a->free_count && a->block_table && a->held_out && a->free_count_out &&
+                a->granted && a->row_start, "%s: null pointer", who);
+    REQUIRE(fits32({a->batch, a->max_pages, a->n_pages, a->max_rows}), "%s: dimensions are 32-bit numbers", who);
+    REQUIRE(a->max_rows >= 0 && (a->max_rows == 0 || (a->slot_map && a->row_seq && a->row_pos)), "%s: null pointer or negative max_rows", who);
+    REQUIRE(a->max_pages > 0 && a->n_pages > 0, "%s: bad max_pages/n_pages", who);
+    for (uint64_t x : {a->seq_lens, a->n_new, a->held, a->free_pages, a->free_count, a->block_table, a->held_out, a->free_count_out, a->granted,
+                       a->row_start, a->slot_map, a->row_seq, a->row_pos})
+        REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);
+    REQUIRE(a->max_pages * 128 < (1l << 31) && a->n_pages * 128 < (1l << 31), "%s: positions and slots are 32-bit numbers", who);
+    if (a->batch > PLAN_MAX_BATCH) { set_error("%s: at most %d requests per call", who, PLAN_MAX_BATCH); return NOMOS_EUNSUPPORTED; }
+    const auto in = [](uint64_t x) { return static_cast<const int *>(ptr(x)); };
+    const auto io = [](uint64_t x) { return static_cast<int *>(ptr(x)); };
+    return launch_paged_plan(as_stream(stream), in(a->seq_lens), in(a->n_new), in(a->held), io(a->free_pages), in(a->free_count),
+                             io(a->block_table), io(a->held_out), io(a->free_count_out), io(a->granted), io(a->row_start), io(a->slot_map),
+                             io(a->row_seq), io(a->row_pos), (int)a->batch, (int)a->max_pages, (int)a->n_pages, (int)a->max_rows);
+}
+
+static int check_page_pool(const char *who, int64_t nkv, int64_t l_hd, int64_t n_pages) {
     REQUIRE(nkv > 0 && n_pages > 0, "%s: bad nkv/n_pages", who);
     if (l_hd != 128 || nkv > 65535) { set_error("%s: paged caches support head_dim 128", who); return NOMOS_EUNSUPPORTED; }
-    REQUIRE((int64_t)n_pages * 128 < (1l << 31), "%s: slots are 32-bit numbers", who);
+    REQUIRE(n_pages < (1l << 24), "%s: slots are 32-bit numbers", who);
     return NOMOS_OK;
 }
 
-NOMOS_EXPORT int32_t nomos_kv_paged_append_rows_i8(void *stream, uint64_t src_k, uint64_t src_v, uint64_t k_pool, uint64_t v_pool,
-                                                   uint64_t ks_pool, uint64_t vs_pool, uint64_t kb_pool, uint64_t kbs_pool,
-                                                   uint64_t slot_map, int32_t n_rows, int32_t nkv, int32_t l_hd, int32_t l_kvd,
-                                                   int32_t n_pages, int32_t src_type) {
+NOMOS_EXPORT int32_t nomos_kv_paged_append_rows_i8(void *stream, const nomos_kv_rows_t *a) {
     const char *who = "nomos_kv_paged_append_rows_i8";
-    if (n_rows <= 0) return NOMOS_OK;
-    REQUIRE(src_k && src_v && k_pool && v_pool && ks_pool && vs_pool && slot_map, "%s: null pointer", who);
-    REQUIRE((kb_pool != 0) == (kbs_pool != 0), "%s: page bounds need both of their pools", who);
-    int rc = check_page_pool(who, nkv, l_hd, n_pages);
+    REQUIRE_BLOCK(a, nomos_kv_rows_t);
+    if (a->n_rows <= 0) return NOMOS_OK;
+    REQUIRE(a->src_k && a->src_v && a->k_pool && a->v_pool && a->ks_pool && a->vs_pool && a->slot_map, "%s: null pointer", who);
+    REQUIRE((a->kb_pool != 0) == (a->kbs_pool != 0), "%s: page bounds need both of their pools", who);
+    int rc = check_page_pool(who, a->nkv, a->l_hd, a->n_pages);
     if (rc) return rc;
-    REQUIRE((int64_t)l_kvd >= (int64_t)nkv * l_hd, "%s: rows of %d elements, %d apart", who, nkv * l_hd, l_kvd);
-    REQUIRE(src_type == ET_F32 || src_type == ET_BF16, "%s: element type", who);
-    const uint64_t es = src_type == ET_BF16 ? 2 : 4;
-    REQUIRE(aligned(src_k, es) && aligned(src_v, es) && aligned(k_pool, 16) && aligned(v_pool, 16) && aligned(ks_pool, 4) &&
-                aligned(vs_pool, 4) && aligned(kb_pool, 16) && aligned(kbs_pool, 4) && aligned(slot_map, 4), "%s: misaligned buffer", who);
-    return launch_append_slots_i8(as_stream(stream), ptr(src_k), ptr(src_v), ptr(k_pool), ptr(v_pool), ptr(ks_pool), ptr(vs_pool),
-                                  ptr(kb_pool), ptr(kbs_pool), static_cast<const int *>(ptr(slot_map)), n_rows, nkv, l_kvd, n_pages,
-                                  src_type == ET_BF16);
+    REQUIRE(fits32({a->n_rows, a->l_kvd}) && a->l_kvd >= a->nkv * a->l_hd, "%s: rows of %ld elements, %ld apart", who, (long)(a->nkv * a->l_hd),
+            (long)a->l_kvd);
+    REQUIRE(a->n_rows * a->nkv <= (1l << 30), "%s: %ld rows of %ld heads in one call", who, (long)a->n_rows, (long)a->nkv);
+    REQUIRE(a->src_type == ET_F32 || a->src_type == ET_BF16, "%s: element type", who);
+    const uint64_t es = a->src_type == ET_BF16 ? 2 : 4;
+    REQUIRE(aligned(a->src_k, es) && aligned(a->src_v, es) && aligned(a->k_pool, 16) && aligned(a->v_pool, 16) && aligned(a->ks_pool, 4) &&
+                aligned(a->vs_pool, 4) && aligned(a->kb_pool, 16) && aligned(a->kbs_pool, 4) && aligned(a->slot_map, 4), "%s: misaligned buffer", who);
+    return launch_append_slots_i8(as_stream(stream), ptr(a->src_k), ptr(a->src_v), ptr(a->k_pool), ptr(a->v_pool), ptr(a->ks_pool),
+                                  ptr(a->vs_pool), ptr(a->kb_pool), ptr(a->kbs_pool), static_cast<const int *>(ptr(a->slot_map)),
+                                  (int)a->n_rows, (int)a->nkv, (int)a->l_kvd, (int)a->n_pages, a->src_type == ET_BF16);
 }
 
 NOMOS_EXPORT int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks_pool, uint64_t kb_pool, uint64_t kbs_pool,
@@ -766,55 +775,57 @@ NOMOS_EXPORT int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32
     return most;
 }
 
-NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, uint64_t q, uint64_t k_pool, uint64_t v_pool, uint64_t ks_pool,
-                                                uint64_t vs_pool, uint64_t kb_pool, uint64_t kbs_pool, uint64_t block_table,
-                                                uint64_t row_seq, uint64_t row_pos, uint64_t out, uint64_t sel_pages, uint64_t workspace,
-                                                int64_t ws_bytes, int32_t rows, int32_t batch, int32_t nh, int32_t nkv, int32_t kvg,
-                                                int32_t l_hd, int32_t n_pages, int32_t max_pages, int32_t max_len, int32_t top_pages,
-                                                int32_t sink_pages, int32_t local_pages, double softmax_scale, int32_t q_type,
-                                                int32_t out_type) {
+NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_sparse_t *c) {
     const char *who = "nomos_attn_paged_sparse_i8";
-    if (rows <= 0 || batch <= 0 || nh <= 0 || max_len <= 0) return NOMOS_OK;
-    REQUIRE(q && k_pool && v_pool && ks_pool && vs_pool && kb_pool && kbs_pool && block_table && row_seq && row_pos && out && workspace,
-            "%s: null pointer", who);
-    int rc = check_page_pool(who, nkv, l_hd, n_pages);
+    REQUIRE_BLOCK(c, nomos_attn_sparse_t);
+    if (c->rows <= 0 || c->batch <= 0 || c->nh <= 0 || c->max_len <= 0) return NOMOS_OK;
+    REQUIRE(c->q && c->k_pool && c->v_pool && c->ks_pool && c->vs_pool && c->kb_pool && c->kbs_pool && c->block_table && c->row_seq &&
+                c->row_pos && c->out && c->workspace, "%s: null pointer", who);
+    REQUIRE(fits32({c->rows, c->batch, c->nh, c->nkv, c->kvg, c->l_hd, c->n_pages, c->max_pages, c->max_len, c->top_pages, c->sink_pages,
+                    c->local_pages}), "%s: dimensions are 32-bit numbers", who);
+    int rc = check_page_pool(who, c->nkv, c->l_hd, c->n_pages);
     if (rc) return rc;
-    REQUIRE((q_type == ET_F32 || q_type == ET_BF16) && (out_type == ET_F32 || out_type == ET_BF16), "%s: element type", who);
-    REQUIRE(aligned(k_pool, 16) && aligned(v_pool, 16) && aligned(ks_pool, 16) && aligned(vs_pool, 16) && aligned(kb_pool, 16) &&
-                aligned(kbs_pool, 4) && aligned(q, 4) && aligned(out, 4) && aligned(block_table, 4) && aligned(row_seq, 4) &&
-                aligned(row_pos, 4) && aligned(sel_pages, 4) && aligned(workspace, 16), "%s: misaligned buffer", who);
-    REQUIRE(max_pages > 0 && (int64_t)max_pages * 128 >= max_len, "%s: max_len %d exceeds max_pages %d x 128", who, max_len, max_pages);
-    REQUIRE(sink_pages >= 0 && local_pages >= 1 && (int64_t)sink_pages + local_pages <= top_pages,
-            "%s: %d first and %d last pages (at least the row's own) of %d selected", who, sink_pages, local_pages, top_pages);
-    REQUIRE(softmax_scale > 0.0 && softmax_scale <= 3.4e38, "%s: the bounds order pages for a positive softmax scale only", who);
-    if (((int64_t)max_len + 127) / 128 > SELECT_MAX_PAGES && ((int64_t)max_len + 127) / 128 > top_pages) {
+    REQUIRE((c->q_type == ET_F32 || c->q_type == ET_BF16) && (c->out_type == ET_F32 || c->out_type == ET_BF16), "%s: element type", who);
+    REQUIRE(aligned(c->k_pool, 16) && aligned(c->v_pool, 16) && aligned(c->ks_pool, 16) && aligned(c->vs_pool, 16) && aligned(c->kb_pool, 16) &&
+                aligned(c->kbs_pool, 4) && aligned(c->q, 4) && aligned(c->out, 4) && aligned(c->block_table, 4) && aligned(c->row_seq, 4) &&
+                aligned(c->row_pos, 4) && aligned(c->sel_pages, 4) && aligned(c->workspace, 16), "%s: misaligned buffer", who);
+    REQUIRE(c->max_pages > 0 && c->max_pages * 128 >= c->max_len, "%s: max_len %ld exceeds max_pages %ld x 128", who, (long)c->max_len,
+            (long)c->max_pages);
+    REQUIRE(c->sink_pages >= 0 && c->local_pages >= 1 && c->sink_pages + c->local_pages <= c->top_pages,
+            "%s: %ld first and %ld last pages (at least the row's own) of %ld selected", who, (long)c->sink_pages, (long)c->local_pages,
+            (long)c->top_pages);
+    REQUIRE(c->softmax_scale > 0.0 && c->softmax_scale <= 3.4e38, "%s: the bounds order pages for a positive softmax scale only", who);
+    const int rows = (int)c->rows, nh = (int)c->nh, nkv = (int)c->nkv, l_hd = (int)c->l_hd, top = (int)c->top_pages, max_len = (int)c->max_len;
+    const int64_t pages = (c->max_len + 127) / 128;
+    if (pages > SELECT_MAX_PAGES && pages > top) {
         set_error("%s: selection from more than %d pages", who, SELECT_MAX_PAGES);
         return NOMOS_EUNSUPPORTED;
     }
-    const size_t qs = q_type == ET_BF16 ? 2 : 4, os = out_type == ET_BF16 ? 2 : 4;
+    const size_t qs = c->q_type == ET_BF16 ? 2 : 4, os = c->out_type == ET_BF16 ? 2 : 4;
     for (int r0 = 0; r0 < rows; r0 += SPARSE_ROWS) {
         const int nr = std::min(SPARSE_ROWS, rows - r0);
         AttnArgs a;
         SparseWs w;
-        rc = fill_sparse(a, w, who, nr, nh, nkv, kvg, l_hd, n_pages, top_pages, max_len);
+        rc = fill_sparse(a, w, who, nr, nh, nkv, (int)c->kvg, l_hd, (int)c->n_pages, top, max_len);
         if (rc) return rc;
-        if (w.lists + w.lens + w.attn > ws_bytes) {
-            set_error("%s: workspace too small: need %ld bytes, have %ld", who, (long)(w.lists + w.lens + w.attn), (long)ws_bytes);
+        if (w.lists + w.lens + w.attn > c->ws_bytes) {
+            set_error("%s: workspace too small: need %ld bytes, have %ld", who, (long)(w.lists + w.lens + w.attn), (long)c->ws_bytes);
             return NOMOS_ECAPACITY;
         }
         PagedSelect s;
-        s.q = ptr(q + (uint64_t)r0 * nh * l_hd * qs); s.kb_pool = ptr(kb_pool); s.kbs_pool = ptr(kbs_pool);
-        s.block_table = static_cast<const int *>(ptr(block_table));
-        s.row_seq = static_cast<const int *>(ptr(row_seq)) + r0; s.row_pos = static_cast<const int *>(ptr(row_pos)) + r0;
-        s.lists = static_cast<int *>(ptr(workspace)); s.lens = static_cast<int *>(ptr(workspace + w.lists));
-        s.sel = sel_pages ? static_cast<int *>(ptr(sel_pages)) + (size_t)r0 * nkv * top_pages : nullptr;
-        s.q_bf16 = q_type == ET_BF16; s.rows = nr; s.batch = batch; s.nh = nh; s.nkv = nkv; s.kvg = kvg; s.n_pages = n_pages;
-        s.max_pages = max_pages; s.max_len = max_len; s.top = top_pages; s.sink = sink_pages; s.local = local_pages;
-        a.q = s.q; a.k_cache = ptr(k_pool); a.v_cache = ptr(v_pool); a.k_scales = ptr(ks_pool); a.v_scales = ptr(vs_pool);
-        a.out = ptr(out + (uint64_t)r0 * nh * l_hd * os);
+        s.q = ptr(c->q + (uint64_t)r0 * nh * l_hd * qs); s.kb_pool = ptr(c->kb_pool); s.kbs_pool = ptr(c->kbs_pool);
+        s.block_table = static_cast<const int *>(ptr(c->block_table));
+        s.row_seq = static_cast<const int *>(ptr(c->row_seq)) + r0; s.row_pos = static_cast<const int *>(ptr(c->row_pos)) + r0;
+        s.lists = static_cast<int *>(ptr(c->workspace)); s.lens = static_cast<int *>(ptr(c->workspace + w.lists));
+        s.sel = c->sel_pages ? static_cast<int *>(ptr(c->sel_pages)) + (size_t)r0 * nkv * top : nullptr;
+        s.q_bf16 = c->q_type == ET_BF16; s.rows = nr; s.batch = (int)c->batch; s.nh = nh; s.nkv = nkv; s.kvg = (int)c->kvg;
+        s.n_pages = (int)c->n_pages; s.max_pages = (int)c->max_pages; s.max_len = max_len; s.top = top; s.sink = (int)c->sink_pages;
+        s.local = (int)c->local_pages;
+        a.q = s.q; a.k_cache = ptr(c->k_pool); a.v_cache = ptr(c->v_pool); a.k_scales = ptr(c->ks_pool); a.v_scales = ptr(c->vs_pool);
+        a.out = ptr(c->out + (uint64_t)r0 * nh * l_hd * os);
         a.block_table = s.lists; a.seq_lens = s.lens;
-        a.workspace = ptr(workspace + w.lists + w.lens); a.ws_bytes = w.attn;
-        a.softmax_scale = (float)softmax_scale; a.q_type = q_type; a.out_type = out_type;
+        a.workspace = ptr(c->workspace + w.lists + w.lens); a.ws_bytes = w.attn;
+        a.softmax_scale = (float)c->softmax_scale; a.q_type = (int)c->q_type; a.out_type = (int)c->out_type;
         rc = launch_paged_select(as_stream(stream), s);
         if (rc) return rc;
         rc = launch_attn_paged(as_stream(stream), a);
@@ -823,23 +834,23 @@ NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, uint64_t q, uint64
     return NOMOS_OK;
 }
 
-NOMOS_EXPORT int32_t nomos_attn_spec_verify(void *stream, uint64_t target_probs, uint64_t draft_probs, uint64_t draft_tokens, uint64_t n_draft,
-                                            uint64_t u_accept, uint64_t u_sample, uint64_t seq_lens, uint64_t seq_lens_out,
-                                            uint64_t n_accepted, uint64_t out_tokens, int32_t batch, int32_t max_draft, int32_t vocab,
-                                            int64_t p_stride, int64_t q_stride) {
+NOMOS_EXPORT int32_t nomos_attn_spec_verify(void *stream, const nomos_attn_verify_t *a) {
     const char *who = "nomos_attn_spec_verify";
-    if (batch <= 0) return NOMOS_OK;
-    REQUIRE(max_draft >= 0 && vocab > 0, "%s: bad max_draft/vocab", who);
-    REQUIRE(target_probs && u_sample && n_accepted && out_tokens && (max_draft == 0 || (draft_tokens && u_accept)), "%s: null pointer", who);
-    REQUIRE((seq_lens != 0) == (seq_lens_out != 0), "%s: lengths need an input and an output", who);
-    REQUIRE(p_stride >= vocab && (!draft_probs || q_stride >= vocab), "%s: rows of %d probabilities, fewer apart", who, vocab);
-    for (uint64_t x : {target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens})
+    REQUIRE_BLOCK(a, nomos_attn_verify_t);
+    if (a->batch <= 0) return NOMOS_OK;
+    REQUIRE(fits32({a->batch, a->max_draft, a->vocab}) && a->max_draft >= 0 && a->max_draft < 0x7fffffff && a->vocab > 0, "%s: bad max_draft/vocab", who);
+    REQUIRE(a->target_probs && a->u_sample && a->n_accepted && a->out_tokens && (a->max_draft == 0 || (a->draft_tokens && a->u_accept)),
+            "%s: null pointer", who);
+    REQUIRE((a->seq_lens != 0) == (a->seq_lens_out != 0), "%s: lengths need an input and an output", who);
+    REQUIRE(a->p_stride >= a->vocab && (!a->draft_probs || a->q_stride >= a->vocab), "%s: rows of %ld probabilities, fewer apart", who, (long)a->vocab);
+    for (uint64_t x : {a->target_probs, a->draft_probs, a->draft_tokens, a->n_draft, a->u_accept, a->u_sample, a->seq_lens, a->seq_lens_out,
+                       a->n_accepted, a->out_tokens})
         REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);
-    const auto f = [](uint64_t a) { return static_cast<const float *>(ptr(a)); };
-    const auto i = [](uint64_t a) { return static_cast<int *>(ptr(a)); };
-    return launch_spec_verify(as_stream(stream), f(target_probs), max_draft > 0 ? f(draft_probs) : nullptr, i(draft_tokens), i(n_draft),
-                              f(u_accept), f(u_sample), i(seq_lens), i(seq_lens_out), i(n_accepted), i(out_tokens), batch, max_draft, vocab,
-                              p_stride, q_stride);
+    const auto f = [](uint64_t x) { return static_cast<const float *>(ptr(x)); };
+    const auto i = [](uint64_t x) { return static_cast<int *>(ptr(x)); };
+    return launch_spec_verify(as_stream(stream), f(a->target_probs), a->max_draft > 0 ? f(a->draft_probs) : nullptr, i(a->draft_tokens),
+                              i(a->n_draft), f(a->u_accept), f(a->u_sample), i(a->seq_lens), i(a->seq_lens_out), i(a->n_accepted),
+                              i(a->out_tokens), (int)a->batch, (int)a->max_draft, (int)a->vocab, a->p_stride, a->q_stride);
 }
 
 NOMOS_EXPORT int32_t nomos_attn_merge_partials(void *stream, uint64_t partials, int32_t G, int32_t rows, int32_t l_hd,

@@ -29,13 +29,16 @@ struct PlanParams {
 
 struct Pair64 { long long a, b; };
 
-// Inclusive prefix sums of two numbers over the block; tot = the block's sums.  `scratch`: 33 entries.
-__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64 *scratch, Pair64 &tot) {
+// Inclusive prefix sums of two numbers over the block, of which the first `busy` warps have any; tot = the block's sums.
+// `scratch`: 33 entries.
+__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64 *scratch, Pair64 &tot, int busy) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+    if (warp < busy) {                   // (the others hold zeros)
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long a = __shfl_up_sync(0xffffffffu, v.a, o), b = __shfl_up_sync(0xffffffffu, v.b, o);
-        if (lane >= o) { v.a += a; v.b += b; }
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long a = __shfl_up_sync(0xffffffffu, v.a, o), b = __shfl_up_sync(0xffffffffu, v.b, o);
+            if (lane >= o) { v.a += a; v.b += b; }
+        }
     }
     __syncthreads();                     // the scratch may still be read from the previous scan
     if (lane == 31) scratch[warp] = v;
@@ -84,23 +87,27 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     if (threadIdx.x == 0) s_taken = 0;
     const int F = max(0, min(p.free_count[0], p.n_pages));
     const int per = (B + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per, b1 = min(B, b0 + per);
+    const int busy = ((B + per - 1) / per + 31) / 32;
 
-    // rows
+    // rows (and everything else that is read of a request, so that the loads are in flight together)
     long long rows = 0;
-    for (int b = b0; b < b1; ++b) rows += max(p.n_new[b], 0);
+    for (int b = b0; b < b1; ++b) {
+        const int n = p.n_new[b], len = p.seq_lens[b], held = p.held[b];
+        s_upto[b] = n; s_len[b] = max(len, 0); s_held[b] = max(0, min(held, p.max_pages));
+        rows += max(n, 0);
+    }
     Pair64 tot;
-    const Pair64 re = block_scan(Pair64{rows, 0}, scratch, tot);
+    const Pair64 re = block_scan(Pair64{rows, 0}, scratch, tot, busy);
     const int total_rows = (int)min(tot.a, (long long)p.max_rows);
     long long end = re.a - rows, need_sum = 0, rel_sum = 0;
     for (int b = b0; b < b1; ++b) {
-        const int n = p.n_new[b], len = max(p.seq_lens[b], 0), held = max(0, min(p.held[b], p.max_pages));
+        const int n = s_upto[b], len = s_len[b], held = s_held[b];
         end += max(n, 0);
         const long long keys = (long long)len + n;
         const bool fits = n > 0 && end <= p.max_rows && keys <= (long long)p.max_pages * PLAN_PAGE;
         const int need = fits ? max(0, (int)((keys + PLAN_PAGE - 1) / PLAN_PAGE) - held) : 0;
         const int rel = n < 0 ? held : 0;
         s_end[b] = (int)min(end, (long long)p.max_rows);
-        s_len[b] = len;
         s_held[b] = fits ? held : -1 - held;
         s_upto[b] = need;
         s_rel[b] = rel;
@@ -108,7 +115,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         rel_sum += rel;
     }
     // pages: a request's need and release become prefix sums (saturated: a sum beyond the pool is never granted)
-    const Pair64 pr = block_scan(Pair64{need_sum, rel_sum}, scratch, tot);
+    const Pair64 pr = block_scan(Pair64{need_sum, rel_sum}, scratch, tot, busy);
     const int R = (int)min(tot.b, (long long)p.n_pages);
     const long long avail = (long long)F + R;
     long long upto = pr.a - need_sum, rel = pr.b - rel_sum;
@@ -147,19 +154,28 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
 
     // rows: four consecutive ones per thread, one search for the four
     for (long long r0 = 4ll * tid; r0 < p.max_rows; r0 += 4ll * nthreads) {
-        int slot[4], seq[4], pos[4];
-        int b = r0 < total_rows ? first_above(s_end, B, (int)r0) : B, last_b = -1, last_j = -1, page = 0;
+        int slot[4] = {-1, -1, -1, -1}, seq[4] = {-1, -1, -1, -1}, pos[4] = {-1, -1, -1, -1};
+        if (r0 < total_rows) {
+            int b = first_above(s_end, B, (int)r0);
+            const int first = b > 0 ? s_end[b - 1] : 0, at0 = s_len[b] + ((int)r0 - first);
+            if (r0 + 4 <= s_end[b] && at0 % PLAN_PAGE + 4 <= PLAN_PAGE) {     // one request, one page
+                if (s_held[b] >= 0) {
+                    const int s0 = (int)((unsigned)page_of(b, at0 / PLAN_PAGE) * PLAN_PAGE + (unsigned)(at0 % PLAN_PAGE));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int r = (int)min(r0 + k, (long long)p.max_rows - 1);
-            while (b < B && s_end[b] <= r) ++b;
-            slot[k] = seq[k] = pos[k] = -1;
-            if (r < total_rows && b < B && s_held[b] >= 0) {
-                const int at = s_len[b] + (r - (b > 0 ? s_end[b - 1] : 0)), j = at / PLAN_PAGE;
-                if (b != last_b || j != last_j) { page = page_of(b, j); last_b = b; last_j = j; }
-                slot[k] = (int)((unsigned)page * PLAN_PAGE + (unsigned)(at % PLAN_PAGE));
-                seq[k] = b;
-                pos[k] = at;
+                    for (int k = 0; k < 4; ++k) { slot[k] = s0 + k; seq[k] = b; pos[k] = at0 + k; }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = (int)r0 + k;
+                    if (r >= total_rows) break;
+                    while (s_end[b] <= r) ++b;
+                    if (s_held[b] < 0) continue;
+                    const int at = s_len[b] + (r - (b > 0 ? s_end[b - 1] : 0));
+                    slot[k] = (int)((unsigned)page_of(b, at / PLAN_PAGE) * PLAN_PAGE + (unsigned)(at % PLAN_PAGE));
+                    seq[k] = b;
+                    pos[k] = at;
+                }
             }
         }
         if (p.vec && r0 + 4 <= p.max_rows) {
@@ -208,8 +224,13 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
     const size_t smem = (size_t)batch * 5 * sizeof(int);
     cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_MAX_BATCH * 5 * (int)sizeof(int)) : cudaSuccess;
     if (e != cudaSuccess) { set_error("nomos_kv_paged_plan: shared memory: %s", cudaGetErrorString(e)); return NOMOS_ECUDA; }
-    // one CTA while its threads cover the rows in one round, else a cluster of eight
-    const int ctas = max_rows <= 4 * PLAN_THREADS ? 1 : 8;
+    // One CTA while its threads cover the rows in one round; else a cluster of sixteen CTAs of half the threads, eight where the
+    // driver does not allow that: the sums are every CTA's own work, the rows are shared.
+    int ctas = max_rows <= 4 * PLAN_THREADS ? 1 : 16;
+    if (ctas == 16 && cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        ctas = 8;
+    }
     const int most = std::max(batch, (max_rows + 3) / 4);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -218,9 +239,15 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
     attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(ctas > 1 ? PLAN_THREADS : std::min(PLAN_THREADS, (most + 31) / 32 * 32));
+    cfg.blockDim = dim3(ctas > 1 ? PLAN_THREADS / 2 : std::min(PLAN_THREADS, (most + 31) / 32 * 32));
     cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, paged_plan_kernel, p);
+    if (e != cudaSuccess && ctas == 16) {
+        cudaGetLastError();
+        cfg.gridDim = dim3(8);
+        attr[1].val.clusterDim.x = 8;
+        e = cudaLaunchKernelEx(&cfg, paged_plan_kernel, p);
+    }
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) { set_error("nomos_kv_paged_plan: %s", cudaGetErrorString(e)); return NOMOS_ECUDA; }
     return NOMOS_OK;

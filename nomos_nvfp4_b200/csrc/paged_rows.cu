@@ -22,96 +22,136 @@ struct PagedRowsArgs {
     float *ks_pool, *vs_pool;
     const int *slot_map;
     int n_rows, nkv, l_kvd;
-    long n_slots;                        // n_pages * 128: slots outside [0, n_slots) are skipped
+    unsigned n_slots;                    // n_pages * 128 < 2^31: slots outside [0, n_slots) are skipped
 };
 
-constexpr int PR_WARPS = 8;              // rows per block
+constexpr int PR_WARPS = 4;              // warps per block
 
-// A warp per (row, K or V, KV head); lane l holds elements 4l .. 4l + 3: one wide load, one 4-byte store of codes.
-// VEC: rows start on a boundary of four elements; otherwise the same elements one by one.
-template <typename SrcT, bool VEC>
+// Four codes trunc(x * inv +- 0.5) as bytes.  With a finite reciprocal of the row's scale |x * inv| <= 127 (1 + 2^-21), so the
+// clamp of the codec (round_away_clamp) has nothing to do.  The conversion packs two at a time.
+__device__ __forceinline__ uint32_t pack_codes(const float *x, float inv) {
+    int q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float t = __fmul_rn(x[e], inv);
+        q[e] = __float2int_rz(__fadd_rn(t, __uint_as_float((__float_as_uint(t) & 0x80000000u) | 0x3f000000u)));
+    }
+    uint32_t hi, w;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(q[3]), "r"(q[2]));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(q[1]), "r"(q[0]), "r"(hi));
+    return w;
+}
+
+// Half a warp per (row, K or V, KV head): lane l holds elements 8l .. 8l + 7, one or two wide loads and one 8-byte store of
+// codes.  A warp takes 2 * STEPS neighbouring heads (of neighbouring rows, where they run out) and has all their loads in
+// flight before the first use: one division by nkv per warp, 16 .. 128 bytes in flight per lane.
+// VEC: rows start on a boundary of eight elements; otherwise the same elements one by one.
+template <typename SrcT, bool VEC, int STEPS>
 __global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __grid_constant__ PagedRowsArgs a) {
+    const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15, kv = blockIdx.y;
+    const int items = a.n_rows * a.nkv;
+    const int item0 = (blockIdx.x * PR_WARPS + (threadIdx.x >> 5)) * 2 * STEPS;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    const long w = (long)blockIdx.x * PR_WARPS + (threadIdx.x >> 5);
-    if (w >= 2l * a.n_rows * a.nkv) return;
-    const int lane = threadIdx.x & 31;
-    const long t = w >> 1;
-    const int kv = (int)(w & 1), h = (int)(t % a.nkv);
-    const long r = t / a.nkv;
-    const SrcT *src = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + (size_t)r * a.l_kvd + (size_t)h * PR_HD + 4 * lane;
-    float x[4];
-    if constexpr (VEC && sizeof(SrcT) == 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(src);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else if constexpr (VEC) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(src);
-        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
-    } else {
+    if (item0 >= items) return;
+    const SrcT *base = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + 8 * l;
+    int r = item0 / a.nkv, h = item0 - r * a.nkv + half;
+    float x[STEPS][8];
+    unsigned slot[STEPS];                // outside the pool: skipped
+    int head[STEPS];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = load_as_f32(src + k);
+    for (int s = 0; s < STEPS; ++s, h += 2) {
+        while (h >= a.nkv) { h -= a.nkv; ++r; }
+        head[s] = h;
+        slot[s] = 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[s][k] = 0.0f;
+        if (r >= a.n_rows) continue;
+        slot[s] = (unsigned)a.slot_map[r];
+        const SrcT *src = base + (size_t)r * a.l_kvd + h * PR_HD;
+        if constexpr (VEC && sizeof(SrcT) == 4) {
+            const float4 u = reinterpret_cast<const float4 *>(src)[0], v = reinterpret_cast<const float4 *>(src)[1];
+            x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
+            x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
+        } else if constexpr (VEC) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(src);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { x[s][2 * k] = __uint_as_float(w[k] << 16); x[s][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[s][k] = load_as_f32(src + k);
+        }
     }
-    const long slot = a.slot_map[r];
-    if (slot < 0 || slot >= a.n_slots) return;
-    float m = 0.0f;
+    // Row maxima; lane l of a half keeps that of its step l % STEPS, so that the two divisions are done once for all steps.
+    float mine = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(x[k]));
-    m = warp_absmax(m);
-    float scale = __fdiv_rn(m, 127.0f);
+    for (int s = 0; s < STEPS; ++s) {
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[s][k]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (l % STEPS == s) mine = m;
+    }
+    float scale = __fdiv_rn(mine, 127.0f);
     if (scale == 0.0f) scale = 1.0f;
-    const float inv = __fdiv_rn(1.0f, scale);
-    uint32_t codes = 0;
+    const float my_inv = __frcp_rn(scale);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) codes |= ((uint32_t)round_away_clamp(__fmul_rn(x[k], inv), 127) & 0xffu) << (8 * k);
-    const size_t row = ((size_t)(slot / PR_PAGE) * a.nkv + h) * PR_PAGE + (size_t)(slot % PR_PAGE);
-    reinterpret_cast<uint32_t *>((kv ? a.v_pool : a.k_pool) + row * PR_HD)[lane] = codes;
-    if (lane == 0) (kv ? a.vs_pool : a.ks_pool)[row] = scale;
+    for (int s = 0; s < STEPS; ++s) {
+        const float sc = __shfl_sync(0xffffffffu, scale, s, 16), inv = __shfl_sync(0xffffffffu, my_inv, s, 16);
+        if (slot[s] >= a.n_slots) continue;            // the same in all lanes of the half
+        uint32_t codes[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) codes[k] = pack_codes(&x[s][4 * k], inv);
+        if (!(inv <= 3.402823466e38f)) {                              // a scale below 2^-128: the products may be infinite
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                codes[k] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) codes[k] |= ((uint32_t)round_away_clamp(__fmul_rn(x[s][4 * k + e], inv), 127) & 0xffu) << (8 * e);
+            }
+        }
+        const size_t row = ((size_t)(slot[s] / PR_PAGE) * a.nkv + head[s]) * PR_PAGE + (size_t)(slot[s] % PR_PAGE);
+        reinterpret_cast<uint2 *>((kv ? a.v_pool : a.k_pool) + row * PR_HD)[l] = make_uint2(codes[0], codes[1]);
+        if (l == 0) (kv ? a.vs_pool : a.ks_pool)[row] = sc;
+    }
 }
 
 constexpr int PB_THREADS = 256;
 
-// Bounds of one page and head by a block of 256 threads: thread = 16 channels of rows (tid / 8), + 32, + 64, + 96.
+// Bounds of one page and head by a block of 256 threads: warp = 16 rows, lane = four channels, whose largest and smallest
+// values stay in registers; every load of the page is in flight at once.
 __device__ __forceinline__ void page_bounds(const int8_t *k_pool, const float *ks_pool, int8_t *kb_pool, float *kbs_pool, size_t unit,
                                             float (*red)[2][PR_HD], float *s_amax, int *s_bad) {
-    const int tid = threadIdx.x, row0 = tid >> 3, c0 = (tid & 7) * 16, warp = tid >> 5, lane = tid & 31;
-    const uint4 *kp = reinterpret_cast<const uint4 *>(k_pool + unit * PR_PAGE * PR_HD);
-    const float *sp = ks_pool + unit * PR_PAGE;
-    uint4 raw[4];
-    float sc[4];
+    constexpr int RPW = PR_PAGE / (PB_THREADS / 32);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t *kp = reinterpret_cast<const uint32_t *>(k_pool + unit * PR_PAGE * PR_HD) + warp * RPW * 32 + lane;
+    uint32_t raw[RPW];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        raw[i] = __ldcg(kp + (size_t)(row0 + 32 * i) * 8 + (tid & 7));
-        sc[i] = __ldcg(sp + row0 + 32 * i);
-    }
-    bool bad = false;
-    float hi[16], lo[16];
+    for (int i = 0; i < RPW; ++i) raw[i] = __ldcg(kp + 32 * i);
+    const float sc = __ldcg(ks_pool + unit * PR_PAGE + warp * RPW + (lane & (RPW - 1)));
+    const bool bad = !(fabsf(sc) <= 3.402823466e38f);
+    float hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) { hi[e] = -CUDART_INF_F; lo[e] = CUDART_INF_F; }
+    for (int e = 0; e < 4; ++e) { hi[e] = -CUDART_INF_F; lo[e] = CUDART_INF_F; }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bad |= !(fabsf(sc[i]) <= 3.402823466e38f);
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    for (int i = 0; i < RPW; ++i) {
+        const float s = __shfl_sync(0xffffffffu, sc, i);
+        const uint32_t w = raw[i] ^ 0x80808080u;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float v = __fmul_rn((float)(int8_t)(w[e >> 2] >> (8 * (e & 3))), sc[i]);
+        for (int e = 0; e < 4; ++e) {
+            // code + 128 as the low byte of the float 2^23 + code + 128: no conversion instruction (a quarter of the rate)
+            const float c = __uint_as_float(prmt(w, 0x4b000000u, 0x7440u | e)) - 8388736.0f;
+            const float v = __fmul_rn(c, s);
             hi[e] = fmaxf(hi[e], v);
             lo[e] = fminf(lo[e], v);
         }
     }
-    // rows of the warp (lanes 8 apart hold the same channels), then of the eight warps
-#pragma unroll
-    for (int o = 8; o < 32; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            hi[e] = fmaxf(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
-            lo[e] = fminf(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
-        }
     __syncthreads();                     // the scratch may still be read for the block's previous page
     if (tid == 0) { *s_bad = 0; }
-    if (lane < 8)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) { red[warp][0][c0 + e] = hi[e]; red[warp][1][c0 + e] = lo[e]; }
+    reinterpret_cast<float4 *>(red[warp][0])[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+    reinterpret_cast<float4 *>(red[warp][1])[lane] = make_float4(lo[0], lo[1], lo[2], lo[3]);
     __syncthreads();
     if (bad) *s_bad = 1;
     const int side = tid >> 7, d = tid & 127;                         // threads 0..127: hi, 128..255: lo
@@ -146,7 +186,7 @@ struct PageBoundsArgs {
 
 // grid (entry spans, KV heads): a block finds the pages of its span and works them out one after the other.
 __global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_constant__ PageBoundsArgs a) {
-    __shared__ float red[PB_THREADS / 32][2][PR_HD];
+    __shared__ __align__(16) float red[PB_THREADS / 32][2][PR_HD];
     __shared__ float s_amax[PB_THREADS / 32];
     __shared__ int s_bad;
     __shared__ int s_pages[PB_THREADS], s_n;
@@ -169,9 +209,8 @@ __global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_co
 
 static int launch_bounds(cudaStream_t st, const PageBoundsArgs &in, const char *who) {
     PageBoundsArgs a = in;
-    // In a decode step few rows end a page, in a prompt every 128th does: spans short enough that a block rarely finds more
-    // than one, long enough that the blocks that find none are few.
-    a.span = a.slots ? 64 : 1;
+    // In a decode step few rows end a page, in a prompt every 128th does: a block that looks at 128 slots finds about one.
+    a.span = a.slots ? PR_PAGE : 1;
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
@@ -194,17 +233,24 @@ int launch_append_slots_i8(cudaStream_t st, const void *src_k, const void *src_v
                            void *kb_pool, void *kbs_pool, const int *slot_map, int n_rows, int nkv, int l_kvd, int n_pages, int src_bf16) {
     const char *who = "nomos_kv_paged_append_rows_i8";
     PagedRowsArgs a{src_k, src_v, static_cast<int8_t *>(k_pool), static_cast<int8_t *>(v_pool), static_cast<float *>(ks_pool),
-                    static_cast<float *>(vs_pool), slot_map, n_rows, nkv, l_kvd, (long)n_pages * PR_PAGE};
-    const int unit = src_bf16 ? 8 : 16;  // four elements
-    const bool vec = l_kvd % 4 == 0 && ((reinterpret_cast<uintptr_t>(src_k) | reinterpret_cast<uintptr_t>(src_v)) & (unit - 1)) == 0;
+                    static_cast<float *>(vs_pool), slot_map, n_rows, nkv, l_kvd, (unsigned)n_pages * PR_PAGE};
+    const bool vec = l_kvd % 8 == 0 && ((reinterpret_cast<uintptr_t>(src_k) | reinterpret_cast<uintptr_t>(src_v)) & 15) == 0;
+    // Several rows per warp once one each would fill the GPU's warps several times over.
+    const int items = n_rows * nkv;
+    const bool many = items > 2 * 148 * 64;
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((2l * n_rows * nkv + PR_WARPS - 1) / PR_WARPS)); cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
+    const int per_block = PR_WARPS * 2 * (many ? 4 : 1);
+    cfg.gridDim = dim3((unsigned)(((long)items + per_block - 1) / per_block), 2); cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
     cfg.attrs = pdl; cfg.numAttrs = 1;
-    cudaError_t e = src_bf16 ? cudaLaunchKernelEx(&cfg, vec ? append_slots_i8_kernel<__nv_bfloat16, true> : append_slots_i8_kernel<__nv_bfloat16, false>, a)
-                             : cudaLaunchKernelEx(&cfg, vec ? append_slots_i8_kernel<float, true> : append_slots_i8_kernel<float, false>, a);
+    void (*kernel)(PagedRowsArgs) =
+        src_bf16 ? (vec ? (many ? append_slots_i8_kernel<__nv_bfloat16, true, 4> : append_slots_i8_kernel<__nv_bfloat16, true, 1>)
+                        : (many ? append_slots_i8_kernel<__nv_bfloat16, false, 4> : append_slots_i8_kernel<__nv_bfloat16, false, 1>))
+                 : (vec ? (many ? append_slots_i8_kernel<float, true, 4> : append_slots_i8_kernel<float, true, 1>)
+                        : (many ? append_slots_i8_kernel<float, false, 4> : append_slots_i8_kernel<float, false, 1>));
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) { set_error("%s: %s", who, cudaGetErrorString(e)); return NOMOS_ECUDA; }
     if (kb_pool == nullptr) return NOMOS_OK;

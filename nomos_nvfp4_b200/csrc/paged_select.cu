@@ -19,7 +19,7 @@
 namespace nomos {
 
 constexpr int SEL_PAGE = 128, SEL_HD = 128;
-constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32;
+constexpr int SEL_WARPS = 16;            // most warps of a CTA
 constexpr float SEL_FLT_MAX = 3.402823466e38f;
 
 struct SelectParams {
@@ -39,15 +39,23 @@ __device__ __forceinline__ uint32_t score_key(float s) {
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(SEL_THREADS) paged_select_kernel(const __grid_constant__ SelectParams p) {
+// Bounds of 16 pages, as one lane holds them: 64 bytes of page g and of page g + 8 of the step, and their scales.
+struct PageStep {
+    uint4 d[2][4];
+    float t_page[2];
+    bool ok[2];
+};
+
+__global__ void __launch_bounds__(SEL_WARPS * 32, 1) paged_select_kernel(const __grid_constant__ SelectParams p) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ __align__(16) uint32_t keys[];                 // first CTA: a key per page
-    __shared__ __align__(16) int8_t qs[8][2 * SEL_HD];               // per head: max(q^, 0), then min(q^, 0)
+    __shared__ __align__(16) int8_t qs[8][2 * SEL_HD + 16];          // per head: max(q^, 0), then min(q^, 0) (rows 16 bytes apart in the banks)
     __shared__ float qscale[8];
     __shared__ uint2 s_count[2][SEL_WARPS];
+    __shared__ uint32_t s_range[2][SEL_WARPS];
     const int rank = blockIdx.x, C = gridDim.x, h = blockIdx.y, row = blockIdx.z;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nthreads = blockDim.x, nwarps = nthreads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const size_t unit = (size_t)row * p.nkv + h;
@@ -64,17 +72,41 @@ __global__ void __launch_bounds__(SEL_THREADS) paged_select_kernel(const __grid_
     if (rank == 0 && threadIdx.x == 0) p.lens[unit] = (min(n, p.top) - 1) * SEL_PAGE + pos % SEL_PAGE + 1;
     if (n <= p.top) {                    // all of them
         if (rank == 0)
-            for (int i = threadIdx.x; i < p.top; i += SEL_THREADS) {
+            for (int i = threadIdx.x; i < p.top; i += nthreads) {
                 if (i < n) list[i] = table[i];
                 if (sel) sel[i] = i < n ? i : -1;
             }
         return;
     }
-    // ---- the group's queries, one warp per head
-    if (warp < 8) {
+    // every CTA of the cluster is running before anyone writes to the first one's shared memory; asked for here, waited for there
+    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    // ---- bounds of the first step's pages: on their way while the query is prepared.  The 256 codes of a page meet the 256 of
+    // the query in any order, as long as both use the same one: lane (g, t) takes bytes [64 j + 16 t, + 16) of page g (and
+    // g + 8) with one wide load each and feeds its words to the operand positions of two instructions; the query's words go
+    // the same way.
+    const int g = lane >> 2, t = lane & 3;
+    const int steps = (n + 15) / 16, stride = C * nwarps;
+    auto load_step = [&](int s, PageStep &x) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int i = 16 * s + g + 8 * k;
+            const int page = i < n ? table[i] : -1;
+            x.ok[k] = page >= 0 && page < p.n_pages;
+            const size_t u = (size_t)(x.ok[k] ? page : 0) * p.nkv + h;
+            const uint4 *src = reinterpret_cast<const uint4 *>(p.kb_pool + u * 2 * SEL_HD) + t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.d[k][j] = src[4 * j];
+            x.t_page[k] = p.kbs_pool[u];
+        }
+    };
+    PageStep cur;
+    int s = rank * nwarps + warp;
+    if (s < steps) load_step(s, cur);
+    // ---- the group's queries, a warp per head
+    for (int j = warp; j < 8; j += nwarps) {
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (warp < p.kvg) {
-            const size_t at = ((size_t)row * p.nh + h * p.kvg + warp) * SEL_HD + lane;
+        if (j < p.kvg) {
+            const size_t at = ((size_t)row * p.nh + h * p.kvg + j) * SEL_HD + lane;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float v = p.q_bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p.q)[at + 32 * k] << 16)
@@ -89,105 +121,125 @@ __global__ void __launch_bounds__(SEL_THREADS) paged_select_kernel(const __grid_
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int c = round_away_clamp(__fmul_rn(x[k], inv), 127);
-            qs[warp][lane + 32 * k] = (int8_t)max(c, 0);
-            qs[warp][SEL_HD + lane + 32 * k] = (int8_t)min(c, 0);
+            qs[j][lane + 32 * k] = (int8_t)max(c, 0);
+            qs[j][SEL_HD + lane + 32 * k] = (int8_t)min(c, 0);
         }
-        if (lane == 0) qscale[warp] = scale;
+        if (lane == 0) qscale[j] = scale;
     }
-    cluster.sync();                      // and every CTA of the cluster is running: its shared memory may be written
-    // ---- scores: 16 pages per warp and step.  The 256 codes of a page meet the 256 of the query in any order, as long as
-    // both use the same one: lane (g, t) takes bytes [64 j + 16 t, + 16) of page g (and g + 8) with one wide load each and
-    // feeds its words to the operand positions of two instructions; the query's words go the same way.
+    __syncthreads();
+    if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    // ---- scores: 16 pages per warp and step, the next step's bounds requested before this one's are used
     {
-        const int g = lane >> 2, t = lane & 3;
         uint4 qf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[j] = *reinterpret_cast<const uint4 *>(&qs[g][64 * j + 16 * t]);
         const bool c0_ok = 2 * t < p.kvg, c1_ok = 2 * t + 1 < p.kvg;
         const float s0 = qscale[2 * t], s1 = qscale[2 * t + 1];
-        uint32_t *out = cluster.map_shared_rank(keys, 0);
-        const int steps = (n + 15) / 16;
-        for (int s = rank * SEL_WARPS + warp; s < steps; s += C * SEL_WARPS) {
-            uint4 d[2][4];
-            float t_page[2];
-            bool ok[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int i = 16 * s + g + 8 * k;
-                const int page = i < n ? table[i] : -1;
-                ok[k] = page >= 0 && page < p.n_pages;
-                const size_t u = (size_t)(ok[k] ? page : 0) * p.nkv + h;
-                const uint4 *src = reinterpret_cast<const uint4 *>(p.kb_pool + u * 2 * SEL_HD) + t;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) d[k][j] = src[4 * j];
-                t_page[k] = p.kbs_pool[u];
-            }
+        uint32_t *out = C > 1 ? cluster.map_shared_rank(keys, 0) : keys;
+        while (s < steps) {
+            const int s_next = s + stride;
+            PageStep next;
+            if (s_next < steps) load_step(s_next, next);
             int acc[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t a0[4] = {d[0][j].x, d[1][j].x, d[0][j].y, d[1][j].y};
+                const uint32_t a0[4] = {cur.d[0][j].x, cur.d[1][j].x, cur.d[0][j].y, cur.d[1][j].y};
                 mma_s8s8(acc, a0, qf[j].x, qf[j].y);
-                const uint32_t a1[4] = {d[0][j].z, d[1][j].z, d[0][j].w, d[1][j].w};
+                const uint32_t a1[4] = {cur.d[0][j].z, cur.d[1][j].z, cur.d[0][j].w, cur.d[1][j].w};
                 mma_s8s8(acc, a1, qf[j].z, qf[j].w);
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 // keys order like scores: the maximum over the heads is taken of the keys
                 uint32_t key = 0;
-                if (c0_ok) key = score_key(__fmul_rn(__fmul_rn((float)acc[2 * k], t_page[k]), s0));
-                if (c1_ok) key = max(key, score_key(__fmul_rn(__fmul_rn((float)acc[2 * k + 1], t_page[k]), s1)));
+                if (c0_ok) key = score_key(__fmul_rn(__fmul_rn((float)acc[2 * k], cur.t_page[k]), s0));
+                if (c1_ok) key = max(key, score_key(__fmul_rn(__fmul_rn((float)acc[2 * k + 1], cur.t_page[k]), s1)));
                 key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
                 key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
                 const int i = 16 * s + g + 8 * k;
                 if (t == 0 && i < n) {
-                    if (!ok[k]) key = 0;                              // no such page in the pool: last of all
+                    if (!cur.ok[k]) key = 0;                          // no such page in the pool: last of all
                     if (i < p.sink || i >= n - p.local) key = 0xffffffffu;
                     out[i] = key;
                 }
             }
+            s = s_next;
+            cur = next;
         }
     }
-    cluster.sync();
-    if (rank != 0) return;
-    // ---- the top-th largest key: two bits per round, from the top; counts of three candidates at once
-    const int span = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32;   // keys of a warp, neighbouring
-    const int w0 = warp * span, w1 = min(n, w0 + span);
-    uint32_t thr = 0;
-#pragma unroll 1
-    for (int bit = 30, it = 0; bit >= 0; bit -= 2, ++it) {
-        const uint32_t t1 = thr | (1u << bit), t2 = thr | (2u << bit), t3 = thr | (3u << bit);
-        uint32_t c12 = 0, c3 = 0;
-        for (int i = w0 + lane; i < w1; i += 32) {
-            const uint32_t k = keys[i];
-            c12 += (k >= t1 ? 1u : 0u) + (k >= t2 ? 0x10000u : 0u);
-            c3 += k >= t3;
-        }
-        c12 = __reduce_add_sync(0xffffffffu, c12);
-        c3 = __reduce_add_sync(0xffffffffu, c3);
-        if (lane == 0) s_count[it & 1][warp] = make_uint2(c12, c3);
+    if (C > 1) {
+        cluster.sync();
+        if (rank != 0) return;
+    } else {
         __syncthreads();
-        uint32_t n1 = 0, n2 = 0, n3 = 0;
-#pragma unroll
-        for (int k = 0; k < SEL_WARPS; ++k) {
-            const uint2 c = s_count[it & 1][k];
-            n1 += c.x & 0xffffu; n2 += c.x >> 16; n3 += c.y;
-        }
-        thr = n3 >= (uint32_t)p.top ? t3 : n2 >= (uint32_t)p.top ? t2 : n1 >= (uint32_t)p.top ? t1 : thr;
     }
+    // ---- the top-th largest key, two bits per round from the highest one in which the keys differ; counts of three candidates
+    // at once.  A warp owns neighbouring keys, the first 8 of each lane in registers.  Ends as soon as exactly `top` keys
+    // reach the candidate: a dozen bits tell most sets of pages apart.
+    constexpr int KR = 8;
+    const int span = ((n + nwarps - 1) / nwarps + 31) / 32 * 32;
+    const int w0 = warp * span, w1 = min(n, w0 + span);
+    uint32_t kreg[KR];
+    uint32_t lo = 0xffffffffu, hi = 0;   // range of the keys that are not forced
+#pragma unroll
+    for (int j = 0; j < KR; ++j) {
+        const int i = w0 + 32 * j + lane;
+        kreg[j] = i < w1 ? keys[i] : 0u;
+        if (i < w1 && kreg[j] != 0xffffffffu) { lo = min(lo, kreg[j]); hi = max(hi, kreg[j]); }
+    }
+    for (int i = w0 + 32 * KR + lane; i < w1; i += 32)
+        if (keys[i] != 0xffffffffu) { lo = min(lo, keys[i]); hi = max(hi, keys[i]); }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) { s_range[0][warp] = lo; s_range[1][warp] = hi; }
+    __syncthreads();
+    for (int k = 0; k < nwarps; ++k) { lo = min(lo, s_range[0][k]); hi = max(hi, s_range[1][k]); }
+    // all keys that are not forced agree above `bit`; the forced ones (fewer than top, or all that is wanted) lie above them
+    const int bits = lo < hi ? 32 - __clz(lo ^ hi) : 0;
+    uint32_t thr = bits == 32 ? 0u : (hi >> bits) << bits;
+    const uint32_t want = (uint32_t)p.top;
+    if (p.sink + p.local == p.top) thr = 0xffffffffu;                 // only the forced ones
+    else {
+#pragma unroll 1
+        for (int bit = (bits + 1) / 2 * 2 - 2, it = 0; bit >= 0; bit -= 2, ++it) {
+            const uint32_t t1 = thr | (1u << bit), t2 = thr | (2u << bit), t3 = thr | (3u << bit);
+            uint32_t c12 = 0, c3 = 0;
+            auto count = [&](uint32_t k) {
+                c12 += (k >= t1 ? 1u : 0u) + (k >= t2 ? 0x10000u : 0u);
+                c3 += k >= t3 ? 1u : 0u;
+            };
+#pragma unroll
+            for (int j = 0; j < KR; ++j)
+                if (32 * j < span) count(kreg[j]);                    // (the fill, 0, reaches no candidate)
+            for (int i = w0 + 32 * KR + lane; i < w1; i += 32) count(keys[i]);
+            c12 = __reduce_add_sync(0xffffffffu, c12);
+            c3 = __reduce_add_sync(0xffffffffu, c3);
+            if (lane == 0) s_count[it & 1][warp] = make_uint2(c12, c3);
+            __syncthreads();
+            uint2 c = lane < nwarps ? s_count[it & 1][lane] : make_uint2(0, 0);
+            const uint32_t n1 = __reduce_add_sync(0xffffffffu, c.x & 0xffffu), n2 = __reduce_add_sync(0xffffffffu, c.x >> 16),
+                           n3 = __reduce_add_sync(0xffffffffu, c.y);
+            uint32_t reach = 0;
+            if (n3 >= want) { thr = t3; reach = n3; }
+            else if (n2 >= want) { thr = t2; reach = n2; }
+            else if (n1 >= want) { thr = t1; reach = n1; }
+            if (reach == want) break;
+        }
+    }
+    __syncthreads();                     // s_count is written again
     // ---- everything above it, and as many equal to it, from the front, as are still wanted
     uint32_t above = 0, equal = 0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t k = keys[i];
-        above += k > thr;
-        equal += k == thr;
-    }
+    auto tally = [&](uint32_t k) { above += k > thr; equal += k == thr; };
+#pragma unroll
+    for (int j = 0; j < KR; ++j)
+        if (w0 + 32 * j + lane < w1) tally(kreg[j]);
+    for (int i = w0 + 32 * KR + lane; i < w1; i += 32) tally(keys[i]);
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) s_count[0][warp] = make_uint2(above, equal);
     __syncthreads();
     int above_all = 0, a0 = 0, e0 = 0;   // of all warps; of the warps before this one
-#pragma unroll
-    for (int k = 0; k < SEL_WARPS; ++k) {
+    for (int k = 0; k < nwarps; ++k) {
         const uint2 c = s_count[0][k];
         above_all += (int)c.x;
         a0 += k < warp ? (int)c.x : 0;
@@ -219,17 +271,22 @@ int launch_paged_select(cudaStream_t st, const PagedSelect &s) {
     SelectParams p{static_cast<const uint8_t *>(s.q), static_cast<const int8_t *>(s.kb_pool), static_cast<const float *>(s.kbs_pool),
                    s.block_table, s.row_seq, s.row_pos, s.lists, s.lens, s.sel, s.q_bf16, s.batch, s.nh, s.nkv, s.kvg, s.n_pages,
                    s.max_pages, s.max_len, s.top, s.sink, s.local};
-    // CTAs per unit: enough to fill the GPU twice over, at most the portable cluster size, none without a step of pages per warp
+    // CTAs per unit: enough to fill the GPU, at most the portable cluster size, none without a step of 16 pages per warp
     const long units = (long)s.rows * s.nkv;
+    const int steps = (pages + 15) / 16;
     int ctas = 8;
-    while (ctas > 1 && (ctas * units > 4 * 148 || ctas * SEL_WARPS * 16 > pages)) ctas /= 2;
+    while (ctas > 1 && (ctas * units > 2 * 148 || ctas * SEL_WARPS > steps)) ctas /= 2;
+    // warps of a CTA: one step each, at least four (the selection's and the query's work); fewer where there are more units than
+    // the SMs hold at sixteen warps
+    int warps = 4;
+    while (warps < SEL_WARPS && warps * ctas < steps && 2 * warps * ctas * units <= 148 * SEL_WARPS) warps *= 2;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, s.nkv, s.rows); cfg.blockDim = dim3(SEL_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = dim3(ctas, s.nkv, s.rows); cfg.blockDim = dim3(warps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cfg.attrs = attr; cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, paged_select_kernel, p);
     if (e == cudaSuccess) e = cudaGetLastError();

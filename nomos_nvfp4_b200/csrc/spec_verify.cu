@@ -15,7 +15,7 @@
 
 namespace nomos {
 
-constexpr int SV_THREADS = 512, SV_WARPS = SV_THREADS / 32;
+constexpr int SV_THREADS = 256, SV_WARPS = SV_THREADS / 32;
 
 struct SpecVerifyArgs {
     const float *p, *q;                  // [batch][max_draft + 1][p_stride], [batch][max_draft][q_stride] or nullptr
@@ -27,11 +27,12 @@ struct SpecVerifyArgs {
     long p_stride, q_stride;
 };
 
-// W of a weight d = p - q in 64 bits.  6 + d lies in [4, 8), whose doubles are 2^-50 apart: the addition rounds d to whole
-// units and the difference of the bit patterns is their number.  (The conversion instruction to 64-bit integers is slower.)
-__device__ __forceinline__ unsigned long long whole_weight(double d) {
-    const long long u = __double_as_longlong(__dadd_rn(fmin(d, 1.0), 6.0)) - __double_as_longlong(6.0);
-    return d > 0.0 ? (unsigned long long)u : 0ull;                   // NaN counts as nothing
+// Adds the whole weight of max(p - q, 0) to a sum.  6 + (p - q) lies in [4, 8), whose doubles are 2^-50 apart: the addition
+// rounds to whole units, and the bit pattern less that of 6.0 (whose low word is zero) is their number.  (A conversion to a
+// 64-bit integer is slower.)  p above 1 counts as 1, NaN as nothing.
+__device__ __forceinline__ void add_weight(unsigned long long &sum, float p, float q) {
+    const long long u = __double_as_longlong(__dadd_rn(__dsub_rn((double)fminf(p, 1.0f), (double)q), 6.0));
+    if (p > q) sum += (unsigned long long)(u - 0x4018000000000000ll);
 }
 
 // One row's weights: target row, drafter row (nullptr: none), and the index whose drafter probability is 1 (a drafter that
@@ -39,9 +40,10 @@ __device__ __forceinline__ unsigned long long whole_weight(double d) {
 struct RowWeights {
     const float *p, *q;
     int one;
-    __device__ __forceinline__ unsigned long long at(int i) const { return of(p[i], q ? q[i] : 0.0f, i); }
-    __device__ __forceinline__ unsigned long long of(float pv, float qv, int i) const {
-        return whole_weight((double)pv - (i == one ? 1.0 : (double)qv));
+    __device__ __forceinline__ unsigned long long at(int i) const {
+        unsigned long long w = 0;
+        add_weight(w, p[i], q ? q[i] : i == one ? 1.0f : 0.0f);
+        return w;
     }
 };
 
@@ -51,26 +53,50 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
     return v;
 }
 
-// Sum over [i0, i1) by one warp; float4 loads where both rows allow them.
-__device__ __forceinline__ unsigned long long warp_range(const RowWeights &w, int i0, int i1, bool vec, int lane) {
+// Sum over [i0, i1) by one warp, where p + i0 is a 16-byte boundary: batches of 512 elements, every load of a batch in flight
+// before the first weight.  Q: 0 no drafter row, 1 drafter row on the same boundary, 2 drafter row anywhere.
+template <int Q>
+__device__ __forceinline__ unsigned long long warp_range(const RowWeights &w, int i0, int i1, int lane) {
+    constexpr int U = 4;
     unsigned long long s = 0;
-    if (vec) {                           // i0 is a multiple of 4
-        int i = i0 + 4 * lane;
-#pragma unroll 4
-        for (; i + 3 < i1; i += 128) {
-            const float4 pv = *reinterpret_cast<const float4 *>(w.p + i);
-            const float4 qv = w.q ? *reinterpret_cast<const float4 *>(w.q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            s += w.of(pv.x, qv.x, i) + w.of(pv.y, qv.y, i + 1) + w.of(pv.z, qv.z, i + 2) + w.of(pv.w, qv.w, i + 3);
+    for (int i = i0 + 4 * lane; i < i1; i += 128 * U) {
+        float4 pv[U], qv[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int j = i + 128 * k;
+            pv[k] = qv[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (j + 4 <= i1) {
+                pv[k] = __ldcs(reinterpret_cast<const float4 *>(w.p + j));
+                if constexpr (Q == 1) qv[k] = __ldcs(reinterpret_cast<const float4 *>(w.q + j));
+                if constexpr (Q == 2) qv[k] = make_float4(w.q[j], w.q[j + 1], w.q[j + 2], w.q[j + 3]);
+            } else if (j < i1) {                                      // the one lane whose four elements the end cuts
+                pv[k].x = w.p[j];
+                if (j + 1 < i1) pv[k].y = w.p[j + 1];
+                if (j + 2 < i1) pv[k].z = w.p[j + 2];
+                if constexpr (Q != 0) {
+                    qv[k].x = w.q[j];
+                    if (j + 1 < i1) qv[k].y = w.q[j + 1];
+                    if (j + 2 < i1) qv[k].z = w.q[j + 2];
+                }
+            }
         }
-        for (; i < i1; ++i) s += w.at(i);                             // the one lane whose four elements the end cuts
-    } else {
-#pragma unroll 4
-        for (int i = i0 + lane; i < i1; i += 32) s += w.at(i);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if constexpr (Q == 0) {
+                const int d = w.one - (i + 128 * k);                  // (a drafted token's own place: its probability counts 1)
+                if ((unsigned)d < 4u) {
+                    qv[k].x = d == 0 ? 1.0f : 0.0f; qv[k].y = d == 1 ? 1.0f : 0.0f;
+                    qv[k].z = d == 2 ? 1.0f : 0.0f; qv[k].w = d == 3 ? 1.0f : 0.0f;
+                }
+            }
+            add_weight(s, pv[k].x, qv[k].x); add_weight(s, pv[k].y, qv[k].y);
+            add_weight(s, pv[k].z, qv[k].z); add_weight(s, pv[k].w, qv[k].w);
+        }
     }
     return warp_sum(s);
 }
 
-__global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const __grid_constant__ SpecVerifyArgs a) {
+__global__ void __launch_bounds__(SV_THREADS, 4) spec_verify_kernel(const __grid_constant__ SpecVerifyArgs a) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ unsigned long long s_warp[2][SV_WARPS], s_total[2], s_scan[SV_WARPS];
@@ -79,6 +105,7 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const __grid_co
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int b = blockIdx.y, rank = blockIdx.x, C = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = min(a.n_draft ? a.n_draft[b] : a.max_draft, a.max_draft);
+    const float u_sample = a.u_sample[b];
     if (n < 0) return;                   // an idle entry of a padded batch; the whole cluster leaves
     // ---- how many drafts stand: every CTA of the cluster finds out for itself
     if (warp == 0) {
@@ -107,15 +134,23 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const __grid_co
     w.p = a.p + ((size_t)b * (a.max_draft + 1) + acc) * a.p_stride;
     w.q = acc < n && a.q ? a.q + ((size_t)b * a.max_draft + acc) * a.q_stride : nullptr;
     w.one = acc < n && !a.q ? a.tokens[(size_t)b * a.max_draft + acc] : -1;
-    const bool vec = ((reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) & 15) == 0;
-    // stretch of this warp: [i0, i1) of the vocabulary, in multiples of four
+    // stretch of this warp: [i0, i1) of the vocabulary, cut where the target row crosses 16-byte boundaries (`lead` elements
+    // precede the first one; they belong to the first warp)
+    const int lead = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(w.p) & 15)) & 15) / 4);
     const int per = (int)((((long)a.vocab + (long)C * SV_WARPS - 1) / ((long)C * SV_WARPS) + 3) / 4 * 4);
+    const auto cut = [&](long unit) { return unit == 0 ? 0 : (int)min(unit * per + lead, (long)a.vocab); };
     const long unit = (long)rank * SV_WARPS + warp;
-    const int i0 = (int)min(unit * per, (long)a.vocab), i1 = (int)min(unit * per + per, (long)a.vocab);
+    const int i0 = cut(unit), i1 = unit == (long)C * SV_WARPS - 1 ? a.vocab : cut(unit + 1);
 
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {
-        const unsigned long long mine = warp_range(w, i0, i1, vec, lane);
+        unsigned long long mine = 0;
+        const int v0 = unit == 0 ? lead : i0;
+        if (!w.q) mine = warp_range<0>(w, v0, i1, lane);
+        else if (((reinterpret_cast<uintptr_t>(w.q + v0)) & 15) == 0) mine = warp_range<1>(w, v0, i1, lane);
+        else mine = warp_range<2>(w, v0, i1, lane);
+        if (unit == 0)
+            for (int i = 0; i < lead; ++i) mine += w.at(i);
         if (lane == 0) s_warp[round][warp] = mine;
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -136,15 +171,15 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const __grid_co
             continue;
         }
         if (total > 0) {
-            const long long t0 = (long long)floor(__dmul_rn((double)a.u_sample[b], (double)total));
+            const long long t0 = (long long)floor(__dmul_rn((double)u_sample, (double)total));
             const unsigned long long T = (unsigned long long)max(0ll, min(t0, (long long)total - 1));
             if (T >= before && T < before + s_total[round]) {         // uniform over the CTA
                 unsigned long long base = before;
                 int k = 0;
                 while (k < SV_WARPS - 1 && T >= base + s_warp[round][k]) base += s_warp[round][k++];
                 // the k-th warp's stretch again, by the whole CTA: `each` neighbouring elements per thread
-                const long u0 = ((long)rank * SV_WARPS + k) * per;
-                const int j0 = (int)min(u0, (long)a.vocab), j1 = (int)min(u0 + per, (long)a.vocab);
+                const long u0 = (long)rank * SV_WARPS + k;
+                const int j0 = cut(u0), j1 = u0 == (long)C * SV_WARPS - 1 ? a.vocab : cut(u0 + 1);
                 const int each = (j1 - j0 + SV_THREADS - 1) / SV_THREADS;
                 const int e0 = min(j1, j0 + (int)threadIdx.x * each), e1 = min(j1, e0 + each);
                 unsigned long long s = 0;
@@ -193,10 +228,10 @@ int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const in
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    // as many CTAs per sequence as fill the GPU about twice over, at most the portable cluster size
+    // As many CTAs per sequence as are resident at once (four of 256 threads per SM), at most the portable cluster size, and
+    // none without a batch of elements for each of its warps.
     int ctas = 8;
-    while (ctas > 1 && (long)ctas * std::min(batch, 65535) > 2 * 148 * 2) ctas /= 2;
-    while (ctas > 1 && vocab < ctas * SV_THREADS * 4) ctas /= 2;
+    while (ctas > 1 && ((long)ctas * std::min(batch, 65535) > 4 * 148 || vocab < ctas * SV_WARPS * 512)) ctas /= 2;
     attr[1].val.clusterDim.x = ctas;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(SV_THREADS); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;

@@ -42,11 +42,24 @@ def _addr(x) -> int:
 
 def _stream(stream) -> C.c_void_p:
     if stream is None:
-        import torch
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        return C.c_void_p(_current_stream())
     if isinstance(stream, int):
         return C.c_void_p(stream)
     return C.c_void_p(stream.cuda_stream)
+
+
+_RAW_STREAM = None
+
+
+def _current_stream() -> int:
+    """torch's current stream on the current device.  The stream object that torch.cuda.current_stream() builds costs 3 us, most of
+    a small call; where torch offers the bare handle (0.1 us) that is taken."""
+    global _RAW_STREAM
+    import torch
+    if _RAW_STREAM is None:
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _RAW_STREAM = (lambda: raw(torch.cuda.current_device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
+    return _RAW_STREAM()
 
 
 def _check(status: int) -> None:
@@ -319,23 +332,26 @@ def kv_paged_append_quant_i8(stream, src_k, src_v, k_pool, v_pool, ks_pool, vs_p
         _addr(block_table), _addr(positions), batch, nkv, l_hd, l_kvd, max_pages))
 
 
+_PLAN, _ROWS, _SPARSE, _VERIFY = (_lib.packer(b) for b in (_lib.KvPlan, _lib.KvRows, _lib.AttnSparse, _lib.AttnVerify))
+
+
 def kv_paged_plan(stream, seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start,
                   slot_map, row_seq, row_pos, *, batch, max_pages, n_pages, max_rows):
     """Block tables and slot maps of a step from request lengths, all int32 on the GPU; see include/nomos_attn.h.
     ``n_new`` < 0 hands a finished request's pages back; ``granted`` tells which requests got their pages."""
-    _check(_lib.lib().nomos_kv_paged_plan(
-        _stream(stream), _addr(seq_lens), _addr(n_new), _addr(held), _addr(free_pages), _addr(free_count), _addr(block_table), _addr(held_out),
+    _check(_lib.lib().nomos_kv_paged_plan(_stream(stream), _PLAN.pack(
+        _PLAN.size, _addr(seq_lens), _addr(n_new), _addr(held), _addr(free_pages), _addr(free_count), _addr(block_table), _addr(held_out),
         _addr(free_count_out), _addr(granted), _addr(row_start), _addr(slot_map), _addr(row_seq), _addr(row_pos), batch, max_pages, n_pages,
-        max_rows))
+        max_rows)))
 
 
 def kv_paged_append_rows_i8(stream, src_k, src_v, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, slot_map, *, n_rows, nkv, l_hd, l_kvd,
                             n_pages, src_type=F32):
     """Quantising append of any number of rows by slot map; with ``kb_pool`` / ``kbs_pool`` (else ``None``) also the bounds of
     every page whose last row is among them."""
-    _check(_lib.lib().nomos_kv_paged_append_rows_i8(
-        _stream(stream), _addr(src_k), _addr(src_v), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool),
-        _addr(kbs_pool), _addr(slot_map), n_rows, nkv, l_hd, l_kvd, n_pages, src_type))
+    _check(_lib.lib().nomos_kv_paged_append_rows_i8(_stream(stream), _ROWS.pack(
+        _ROWS.size, _addr(src_k), _addr(src_v), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool), _addr(kbs_pool),
+        _addr(slot_map), n_rows, nkv, l_hd, l_kvd, n_pages, src_type)))
 
 
 def kv_paged_page_bounds_i8(stream, k_pool, ks_pool, kb_pool, kbs_pool, pages, *, n, nkv, l_hd, n_pages):
@@ -356,19 +372,19 @@ def attn_paged_sparse_i8(stream, q, k_pool, v_pool, ks_pool, vs_pool, kb_pool, k
                          softmax_scale=1.0, q_type=F32, out_type=F32):
     """Attention of ``rows`` query rows (decode, verify and prompt rows alike: sequence ``row_seq[r]``, position ``row_pos[r]``)
     over at most ``top_pages`` pages each, selected per row and KV head by a bound on the logits; see include/nomos_attn.h."""
-    _check(_lib.lib().nomos_attn_paged_sparse_i8(
-        _stream(stream), _addr(q), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool), _addr(kbs_pool),
-        _addr(block_table), _addr(row_seq), _addr(row_pos), _addr(out), _addr(sel_pages), _addr(workspace), int(ws_bytes), rows, batch, nh, nkv,
-        kvg, l_hd, n_pages, max_pages, max_len, top_pages, sink_pages, local_pages, float(softmax_scale), q_type, out_type))
+    _check(_lib.lib().nomos_attn_paged_sparse_i8(_stream(stream), _SPARSE.pack(
+        _SPARSE.size, _addr(q), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool), _addr(kbs_pool), _addr(block_table),
+        _addr(row_seq), _addr(row_pos), _addr(out), _addr(sel_pages), _addr(workspace), int(ws_bytes), rows, batch, nh, nkv, kvg, l_hd, n_pages,
+        max_pages, max_len, top_pages, sink_pages, local_pages, softmax_scale, q_type, out_type)))
 
 
 def spec_verify(stream, target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens, *,
                 batch, max_draft, vocab, p_stride, q_stride):
     """Speculative verification from given random numbers: accepted drafts, and the next token from the residual (or, all
     accepted, from the target's last row); see include/nomos_attn.h.  ``draft_probs``, ``n_draft``, ``seq_lens`` may be ``None``."""
-    _check(_lib.lib().nomos_attn_spec_verify(
-        _stream(stream), _addr(target_probs), _addr(draft_probs), _addr(draft_tokens), _addr(n_draft), _addr(u_accept), _addr(u_sample),
-        _addr(seq_lens), _addr(seq_lens_out), _addr(n_accepted), _addr(out_tokens), batch, max_draft, vocab, p_stride, q_stride))
+    _check(_lib.lib().nomos_attn_spec_verify(_stream(stream), _VERIFY.pack(
+        _VERIFY.size, _addr(target_probs), _addr(draft_probs), _addr(draft_tokens), _addr(n_draft), _addr(u_accept), _addr(u_sample),
+        _addr(seq_lens), _addr(seq_lens_out), _addr(n_accepted), _addr(out_tokens), batch, max_draft, vocab, p_stride, q_stride)))
 
 
 class KvRing:

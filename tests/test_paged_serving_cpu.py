@@ -14,6 +14,29 @@ def ops():
     return ops
 
 
+@pytest.mark.parametrize("name,mirror", [("nomos_kv_plan", "KvPlan"), ("nomos_kv_rows", "KvRows"), ("nomos_attn_sparse", "AttnSparse"),
+                                         ("nomos_attn_verify", "AttnVerify")])
+def test_argument_blocks_match_the_header(ops, name, mirror):
+    import ctypes
+    import re
+    from pathlib import Path
+    from nomos_nvfp4_b200 import _lib
+    text = (Path(__file__).resolve().parent.parent / "include" / "nomos_attn.h").read_text()
+    body = re.search(r"typedef struct %s \{(.*?)\} %s_t;" % (name, name), text, flags=re.S).group(1)
+    declared = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        kind, names = decl.split(None, 1)
+        declared += [(n.strip(), kind) for n in names.split(",")]
+    block = getattr(_lib, mirror)
+    kinds = {ctypes.c_uint64: "uint64_t", ctypes.c_int64: "int64_t", ctypes.c_double: "double"}
+    assert declared == [(n, kinds[t]) for n, t in block._fields_]
+    assert _lib.packer(block).size == ctypes.sizeof(block) == 8 * len(declared)
+    fn = {"KvPlan": "nomos_kv_paged_plan", "KvRows": "nomos_kv_paged_append_rows_i8", "AttnSparse": "nomos_attn_paged_sparse_i8",
+          "AttnVerify": "nomos_attn_spec_verify"}[mirror]
+    assert getattr(_lib.lib(), fn)(None, bytes(8 * len(declared))) == -1      # struct_bytes of another version
+    assert getattr(_lib.lib(), fn)(None, None) == -1
+
+
 def refused(ops, status, call, *args, **kw):
     with pytest.raises(ops.NomosError) as e:
         call(*args, **kw)
@@ -25,7 +48,8 @@ def test_plan_refusals(ops):
     for i in range(13):
         refused(ops, -1, ops.kv_paged_plan, 0, *[None if j == i else P for j in range(13)], **kw)
         refused(ops, -1, ops.kv_paged_plan, 0, *[P + 2 if j == i else P for j in range(13)], **kw)
-    for bad in (dict(max_pages=0), dict(n_pages=0), dict(max_rows=-1), dict(max_pages=1 << 24), dict(n_pages=1 << 24)):
+    for bad in (dict(max_pages=0), dict(n_pages=0), dict(max_rows=-1), dict(max_pages=1 << 24), dict(n_pages=1 << 24), dict(batch=1 << 32),
+                dict(max_rows=1 << 31)):
         refused(ops, -1, ops.kv_paged_plan, 0, *[P] * 13, **{**kw, **bad})
     refused(ops, -2, ops.kv_paged_plan, 0, *[P] * 13, **{**kw, "batch": 8193})
     ops.kv_paged_plan(0, *[None] * 13, **{**kw, "batch": 0})
@@ -64,7 +88,7 @@ def test_sparse_refusals(ops):
         refused(ops, -1, ops.attn_paged_sparse_i8, 0, *[P + 2 if j == i else x for j, x in enumerate(good)], **kw)
     for bad in (dict(kvg=3), dict(max_len=16 * 128 + 1), dict(local_pages=0), dict(sink_pages=-1), dict(sink_pages=3), dict(top_pages=2),
                 dict(softmax_scale=0.0), dict(softmax_scale=-1.0), dict(softmax_scale=float("nan")), dict(softmax_scale=float("inf")),
-                dict(q_type=2), dict(out_type=-1), dict(n_pages=0), dict(top_pages=0, sink_pages=0)):
+                dict(q_type=2), dict(out_type=-1), dict(n_pages=0), dict(top_pages=0, sink_pages=0), dict(rows=1 << 40), dict(max_pages=1 << 33)):
         refused(ops, -1, ops.attn_paged_sparse_i8, 0, *good, **{**kw, **bad})
     for bad in (dict(l_hd=256), dict(nh=36, kvg=9)):
         refused(ops, -2, ops.attn_paged_sparse_i8, 0, *good, **{**kw, **bad})
@@ -83,7 +107,7 @@ def test_verify_refusals(ops):
         if i not in optional:                                          # (lengths: one of the two alone is refused)
             refused(ops, -1, ops.spec_verify, 0, *[None if j == i else P for j in range(10)], **kw)
         refused(ops, -1, ops.spec_verify, 0, *[P + 2 if j == i else P for j in range(10)], **kw)
-    for bad in (dict(vocab=0), dict(max_draft=-1), dict(p_stride=99), dict(q_stride=99)):
+    for bad in (dict(vocab=0), dict(max_draft=-1), dict(p_stride=99), dict(q_stride=99), dict(batch=1 << 31), dict(vocab=1 << 32, p_stride=1 << 33, q_stride=1 << 33)):
         refused(ops, -1, ops.spec_verify, 0, *[P] * 10, **{**kw, **bad})
     ops.spec_verify(0, *[None] * 10, **{**kw, "batch": 0})
 
