@@ -21,11 +21,11 @@ struct PagedRowsArgs {
     int8_t *k_pool, *v_pool;
     float *ks_pool, *vs_pool;
     const int *slot_map;
-    int n_rows, nkv, l_kvd;
+    int n_rows, nkv, l_kvd, head_bits;
     unsigned n_slots;                    // n_pages * 128 < 2^31: slots outside [0, n_slots) are skipped
 };
 
-constexpr int PR_WARPS = 4;              // warps per block
+constexpr int PR_WARPS = 8;              // warps per block: sixteen halves
 
 // Four codes trunc(x * inv +- 0.5) as bytes.  With a finite reciprocal of the row's scale |x * inv| <= 127 (1 + 2^-21), so the
 // clamp of the codec (round_away_clamp) has nothing to do.  The conversion packs two at a time.
@@ -43,32 +43,26 @@ __device__ __forceinline__ uint32_t pack_codes(const float *x, float inv) {
 }
 
 // Half a warp per (row, K or V, KV head): lane l holds elements 8l .. 8l + 7, one or two wide loads and one 8-byte store of
-// codes.  A warp takes 2 * STEPS neighbouring heads (of neighbouring rows, where they run out) and has all their loads in
-// flight before the first use: one division by nkv per warp, 16 .. 128 bytes in flight per lane.
+// codes.  The sixteen half warps of a block take the heads of one row (nkv <= 8: of several rows, 2^head_bits half warps
+// each; nkv > 16: sixteen heads per blockIdx.z), so that no index needs a division, and STEPS such sets of rows, all loaded
+// before the first use.
 // VEC: rows start on a boundary of eight elements; otherwise the same elements one by one.
 template <typename SrcT, bool VEC, int STEPS>
 __global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __grid_constant__ PagedRowsArgs a) {
-    const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15, kv = blockIdx.y;
-    const int items = a.n_rows * a.nkv;
-    const int item0 = (blockIdx.x * PR_WARPS + (threadIdx.x >> 5)) * 2 * STEPS;
+    const int hw = threadIdx.x >> 4, l = threadIdx.x & 15, kv = blockIdx.y;
+    const int rows_step = (2 * PR_WARPS) >> a.head_bits;
+    const int r0 = blockIdx.x * (rows_step * STEPS) + (hw >> a.head_bits);
+    const int h = 2 * PR_WARPS * blockIdx.z + (hw & ((1 << a.head_bits) - 1));
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    if (item0 >= items) return;
-    const SrcT *base = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + 8 * l;
-    int r = item0 / a.nkv, h = item0 - r * a.nkv + half;
+    const SrcT *base = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + min(h, a.nkv - 1) * PR_HD + 8 * l;
     float x[STEPS][8];
     unsigned slot[STEPS];                // outside the pool: skipped
-    int head[STEPS];
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s, h += 2) {
-        while (h >= a.nkv) { h -= a.nkv; ++r; }
-        head[s] = h;
-        slot[s] = 0xffffffffu;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[s][k] = 0.0f;
-        if (r >= a.n_rows) continue;
+    for (int s = 0; s < STEPS; ++s) {
+        const int r = min(r0 + s * rows_step, a.n_rows - 1);
         slot[s] = (unsigned)a.slot_map[r];
-        const SrcT *src = base + (size_t)r * a.l_kvd + h * PR_HD;
+        const SrcT *src = base + (size_t)r * a.l_kvd;
         if constexpr (VEC && sizeof(SrcT) == 4) {
             const float4 u = reinterpret_cast<const float4 *>(src)[0], v = reinterpret_cast<const float4 *>(src)[1];
             x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
@@ -100,7 +94,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const float sc = __shfl_sync(0xffffffffu, scale, s, 16), inv = __shfl_sync(0xffffffffu, my_inv, s, 16);
-        if (slot[s] >= a.n_slots) continue;            // the same in all lanes of the half
+        if (slot[s] >= a.n_slots || h >= a.nkv || r0 + s * rows_step >= a.n_rows) continue;   // the same in all lanes of the half
         uint32_t codes[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) codes[k] = pack_codes(&x[s][4 * k], inv);
@@ -112,7 +106,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __
                 for (int e = 0; e < 4; ++e) codes[k] |= ((uint32_t)round_away_clamp(__fmul_rn(x[s][4 * k + e], inv), 127) & 0xffu) << (8 * e);
             }
         }
-        const size_t row = ((size_t)(slot[s] / PR_PAGE) * a.nkv + head[s]) * PR_PAGE + (size_t)(slot[s] % PR_PAGE);
+        const size_t row = ((size_t)(slot[s] / PR_PAGE) * a.nkv + h) * PR_PAGE + (size_t)(slot[s] % PR_PAGE);
         reinterpret_cast<uint2 *>((kv ? a.v_pool : a.k_pool) + row * PR_HD)[l] = make_uint2(codes[0], codes[1]);
         if (l == 0) (kv ? a.vs_pool : a.ks_pool)[row] = sc;
     }
@@ -192,15 +186,19 @@ __global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_co
     __shared__ int s_pages[PB_THREADS], s_n;
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    // Slots: the preceding grid is the append of the same call, which waited for its own predecessor before it let this one be
+    // scheduled.  The slot map is settled then and looked through while the append still runs.  A page list may be the
+    // preceding grid's work.
+    if (!a.slots) asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int i = blockIdx.x * a.span + threadIdx.x;
     if ((int)threadIdx.x < a.span && i < a.n) {
-        const int v = a.list[i];
+        const int v = __ldcg(a.list + i);
         const bool last = !a.slots || (v >= 0 && v % PR_PAGE == PR_PAGE - 1);
         const int page = a.slots ? v / PR_PAGE : v;
         if (last && page >= 0 && page < a.n_pages) s_pages[atomicAdd(&s_n, 1)] = page;   // any order: pages are independent
     }
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");              // (every block: the grid ends after the append)
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     __syncthreads();
     const int n = s_n;
     for (int k = 0; k < n; ++k)
@@ -233,23 +231,24 @@ int launch_append_slots_i8(cudaStream_t st, const void *src_k, const void *src_v
                            void *kb_pool, void *kbs_pool, const int *slot_map, int n_rows, int nkv, int l_kvd, int n_pages, int src_bf16) {
     const char *who = "nomos_kv_paged_append_rows_i8";
     PagedRowsArgs a{src_k, src_v, static_cast<int8_t *>(k_pool), static_cast<int8_t *>(v_pool), static_cast<float *>(ks_pool),
-                    static_cast<float *>(vs_pool), slot_map, n_rows, nkv, l_kvd, (unsigned)n_pages * PR_PAGE};
+                    static_cast<float *>(vs_pool), slot_map, n_rows, nkv, l_kvd, 0, (unsigned)n_pages * PR_PAGE};
+    while (a.head_bits < 4 && (1 << a.head_bits) < nkv) ++a.head_bits;
     const bool vec = l_kvd % 8 == 0 && ((reinterpret_cast<uintptr_t>(src_k) | reinterpret_cast<uintptr_t>(src_v)) & 15) == 0;
-    // Several rows per warp once one each would fill the GPU's warps several times over.
-    const int items = n_rows * nkv;
-    const bool many = items > 2 * 148 * 64;
+    // Two sets of rows per block once one each would fill the GPU's warps several times over.
+    const bool many = (long)n_rows * nkv > 2 * 148 * 64;
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    const int per_block = PR_WARPS * 2 * (many ? 4 : 1);
-    cfg.gridDim = dim3((unsigned)(((long)items + per_block - 1) / per_block), 2); cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
+    const int per_block = ((2 * PR_WARPS) >> a.head_bits) * (many ? 2 : 1);
+    cfg.gridDim = dim3((unsigned)(((long)n_rows + per_block - 1) / per_block), 2, (nkv + 2 * PR_WARPS - 1) / (2 * PR_WARPS));
+    cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
     cfg.attrs = pdl; cfg.numAttrs = 1;
     void (*kernel)(PagedRowsArgs) =
-        src_bf16 ? (vec ? (many ? append_slots_i8_kernel<__nv_bfloat16, true, 4> : append_slots_i8_kernel<__nv_bfloat16, true, 1>)
-                        : (many ? append_slots_i8_kernel<__nv_bfloat16, false, 4> : append_slots_i8_kernel<__nv_bfloat16, false, 1>))
-                 : (vec ? (many ? append_slots_i8_kernel<float, true, 4> : append_slots_i8_kernel<float, true, 1>)
-                        : (many ? append_slots_i8_kernel<float, false, 4> : append_slots_i8_kernel<float, false, 1>));
+        src_bf16 ? (vec ? (many ? append_slots_i8_kernel<__nv_bfloat16, true, 2> : append_slots_i8_kernel<__nv_bfloat16, true, 1>)
+                        : (many ? append_slots_i8_kernel<__nv_bfloat16, false, 2> : append_slots_i8_kernel<__nv_bfloat16, false, 1>))
+                 : (vec ? (many ? append_slots_i8_kernel<float, true, 2> : append_slots_i8_kernel<float, true, 1>)
+                        : (many ? append_slots_i8_kernel<float, false, 2> : append_slots_i8_kernel<float, false, 1>));
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) { set_error("%s: %s", who, cudaGetErrorString(e)); return NOMOS_ECUDA; }
