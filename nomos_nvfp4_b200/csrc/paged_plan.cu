@@ -27,33 +27,31 @@ struct PlanParams {
     int vec;                             // the three row arrays start on 16-byte boundaries
 };
 
-struct Pair64 { long long a, b; };
+struct Sums { long long rows, need, rel; };
 
-// Inclusive prefix sums of two numbers over the block, of which the first `busy` warps have any; tot = the block's sums.
-// `scratch`: 33 entries.
-__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64 *scratch, Pair64 &tot, int busy) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
-    if (warp < busy) {                   // (the others hold zeros)
+__device__ __forceinline__ Sums warp_scan(Sums v, int lane) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long a = __shfl_up_sync(0xffffffffu, v.a, o), b = __shfl_up_sync(0xffffffffu, v.b, o);
-            if (lane >= o) { v.a += a; v.b += b; }
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long a = __shfl_up_sync(0xffffffffu, v.rows, o), b = __shfl_up_sync(0xffffffffu, v.need, o), c = __shfl_up_sync(0xffffffffu, v.rel, o);
+        if (lane >= o) { v.rows += a; v.need += b; v.rel += c; }
     }
-    __syncthreads();                     // the scratch may still be read from the previous scan
+    return v;
+}
+
+// Inclusive prefix sums over the block, of which the first `busy` warps have any; tot = the block's sums.  `scratch`: 32 entries.
+__device__ __forceinline__ Sums block_scan(Sums v, Sums *scratch, Sums &tot, int busy) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+    if (warp < busy) v = warp_scan(v, lane);                          // (the others hold zeros)
     if (lane == 31) scratch[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        Pair64 w = lane < nwarp ? scratch[lane] : Pair64{0, 0};
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long a = __shfl_up_sync(0xffffffffu, w.a, o), b = __shfl_up_sync(0xffffffffu, w.b, o);
-            if (lane >= o) { w.a += a; w.b += b; }
-        }
+        Sums w = lane < nwarp ? scratch[lane] : Sums{0, 0, 0};
+        w = warp_scan(w, lane);
+        __syncwarp();
         scratch[lane] = w;
     }
     __syncthreads();
-    if (warp > 0) { v.a += scratch[warp - 1].a; v.b += scratch[warp - 1].b; }
+    if (warp > 0) { v.rows += scratch[warp - 1].rows; v.need += scratch[warp - 1].need; v.rel += scratch[warp - 1].rel; }
     tot = scratch[31];
     return v;
 }
@@ -79,7 +77,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     int *s_held = s_len + B;             // pages held; -1 - pages: not served in this step
     int *s_upto = s_held + B;            // pages needed up to and including the request
     int *s_rel = s_upto + B;             // pages released up to and including the request
-    __shared__ Pair64 scratch[33];
+    __shared__ Sums scratch[32];
     __shared__ int s_taken;
 
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
@@ -89,46 +87,41 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     const int per = (B + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per, b1 = min(B, b0 + per);
     const int busy = ((B + per - 1) / per + 31) / 32;
 
-    // rows (and everything else that is read of a request, so that the loads are in flight together)
-    long long rows = 0;
+    // Rows, pages needed and pages released, in one scan.  Whether a request's rows end behind max_rows is not known yet: those
+    // that do are a tail of the requests, so what they would need is in no other request's sum.
+    Sums own{0, 0, 0};
     for (int b = b0; b < b1; ++b) {
-        const int n = p.n_new[b], len = p.seq_lens[b], held = p.held[b];
-        s_upto[b] = n; s_len[b] = max(len, 0); s_held[b] = max(0, min(held, p.max_pages));
-        rows += max(n, 0);
-    }
-    Pair64 tot;
-    const Pair64 re = block_scan(Pair64{rows, 0}, scratch, tot, busy);
-    const int total_rows = (int)min(tot.a, (long long)p.max_rows);
-    long long end = re.a - rows, need_sum = 0, rel_sum = 0;
-    for (int b = b0; b < b1; ++b) {
-        const int n = s_upto[b], len = s_len[b], held = s_held[b];
-        end += max(n, 0);
+        const int n = p.n_new[b], len = max(p.seq_lens[b], 0), held = max(0, min(p.held[b], p.max_pages));
         const long long keys = (long long)len + n;
-        const bool fits = n > 0 && end <= p.max_rows && keys <= (long long)p.max_pages * PLAN_PAGE;
+        const bool fits = n > 0 && keys <= (long long)p.max_pages * PLAN_PAGE;
         const int need = fits ? max(0, (int)((keys + PLAN_PAGE - 1) / PLAN_PAGE) - held) : 0;
-        const int rel = n < 0 ? held : 0;
-        s_end[b] = (int)min(end, (long long)p.max_rows);
+        s_end[b] = n;
+        s_len[b] = len;
         s_held[b] = fits ? held : -1 - held;
         s_upto[b] = need;
-        s_rel[b] = rel;
-        need_sum += need;
-        rel_sum += rel;
+        own.rows += max(n, 0);
+        own.need += need;
+        own.rel += n < 0 ? held : 0;
     }
-    // pages: a request's need and release become prefix sums (saturated: a sum beyond the pool is never granted)
-    const Pair64 pr = block_scan(Pair64{need_sum, rel_sum}, scratch, tot, busy);
-    const int R = (int)min(tot.b, (long long)p.n_pages);
+    Sums tot;
+    const Sums upto = block_scan(own, scratch, tot, busy);
+    const int total_rows = (int)min(tot.rows, (long long)p.max_rows);
+    const int R = (int)min(tot.rel, (long long)p.n_pages);
     const long long avail = (long long)F + R;
-    long long upto = pr.a - need_sum, rel = pr.b - rel_sum;
+    // each request's own place in the sums (saturated: a sum beyond the pool is never granted)
+    long long end = upto.rows - own.rows, need_upto = upto.need - own.need, rel = upto.rel - own.rel;
     int taken = 0;
     for (int b = b0; b < b1; ++b) {
-        const int need = s_upto[b];
-        upto += need;
-        rel += s_rel[b];
-        if (s_held[b] >= 0 && need > 0) {
-            if (upto <= avail) taken = (int)upto;                   // upto only grows: what is granted is a prefix
-            else s_held[b] = -1 - s_held[b];
+        const int n = s_end[b], need = s_upto[b], h = s_held[b];
+        end += max(n, 0);
+        need_upto += need;
+        if (n < 0) rel += -1 - h;
+        if (h >= 0) {
+            if (end > p.max_rows || (need > 0 && need_upto > avail)) s_held[b] = -1 - h;
+            else if (need > 0) taken = (int)need_upto;                // it only grows: what is granted is a prefix
         }
-        s_upto[b] = (int)min(upto, 0x7fffffffll);
+        s_end[b] = (int)min(end, (long long)p.max_rows);
+        s_upto[b] = (int)min(need_upto, 0x7fffffffll);
         s_rel[b] = (int)min(rel, 0x7fffffffll);
     }
     if (taken > 0) atomicMax(&s_taken, taken);

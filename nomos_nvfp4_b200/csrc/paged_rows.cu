@@ -42,19 +42,12 @@ __device__ __forceinline__ uint32_t pack_codes(const float *x, float inv) {
     return w;
 }
 
-// Half a warp per (row, K or V, KV head): lane l holds elements 8l .. 8l + 7, one or two wide loads and one 8-byte store of
-// codes.  The sixteen half warps of a block take the heads of one row (nkv <= 8: of several rows, 2^head_bits half warps
-// each; nkv > 16: sixteen heads per blockIdx.z), so that no index needs a division, and STEPS such sets of rows, all loaded
-// before the first use.
+// Half a warp per row of one (K or V, KV head): lane l holds elements 8l .. 8l + 7, one or two wide loads and one 8-byte store of
+// codes.  The half warp takes rows r0, r0 + rows_step, ... (STEPS of them, loaded before the first use).
 // VEC: rows start on a boundary of eight elements; otherwise the same elements one by one.
 template <typename SrcT, bool VEC, int STEPS>
-__global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __grid_constant__ PagedRowsArgs a) {
-    const int hw = threadIdx.x >> 4, l = threadIdx.x & 15, kv = blockIdx.y;
-    const int rows_step = (2 * PR_WARPS) >> a.head_bits;
-    const int r0 = blockIdx.x * (rows_step * STEPS) + (hw >> a.head_bits);
-    const int h = 2 * PR_WARPS * blockIdx.z + (hw & ((1 << a.head_bits) - 1));
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+__device__ __forceinline__ void append_rows(const PagedRowsArgs &a, int kv, int h, int r0, int rows_step) {
+    const int l = threadIdx.x & 15;
     const SrcT *base = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + min(h, a.nkv - 1) * PR_HD + 8 * l;
     float x[STEPS][8];
     unsigned slot[STEPS];                // outside the pool: skipped
@@ -112,12 +105,30 @@ __global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __
     }
 }
 
+// The sixteen half warps of a block take the heads of one row (nkv <= 8: of several rows, 2^head_bits half warps each; nkv > 16:
+// sixteen heads per blockIdx.z), so that no index needs a division, and STEPS such sets of rows.
+template <typename SrcT, bool VEC, int STEPS>
+__global__ void __launch_bounds__(PR_WARPS * 32) append_slots_i8_kernel(const __grid_constant__ PagedRowsArgs a) {
+    const int hw = threadIdx.x >> 4;
+    const int rows_step = (2 * PR_WARPS) >> a.head_bits;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    append_rows<SrcT, VEC, STEPS>(a, blockIdx.y, 2 * PR_WARPS * blockIdx.z + (hw & ((1 << a.head_bits) - 1)),
+                                  blockIdx.x * (rows_step * STEPS) + (hw >> a.head_bits), rows_step);
+}
+
 constexpr int PB_THREADS = 256;
+static_assert(PB_THREADS == PR_WARPS * 32, "the append of a head's rows works its pages' bounds out with the same block");
+struct BoundsScratch {
+    __align__(16) float red[PB_THREADS / 32][2][PR_HD];
+    float amax[PB_THREADS / 32];
+    int bad;
+};
 
 // Bounds of one page and head by a block of 256 threads: warp = 16 rows, lane = four channels, whose largest and smallest
 // values stay in registers; every load of the page is in flight at once.
 __device__ __forceinline__ void page_bounds(const int8_t *k_pool, const float *ks_pool, int8_t *kb_pool, float *kbs_pool, size_t unit,
-                                            float (*red)[2][PR_HD], float *s_amax, int *s_bad) {
+                                            BoundsScratch &sm) {
     constexpr int RPW = PR_PAGE / (PB_THREADS / 32);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t *kp = reinterpret_cast<const uint32_t *>(k_pool + unit * PR_PAGE * PR_HD) + warp * RPW * 32 + lane;
@@ -143,28 +154,51 @@ __device__ __forceinline__ void page_bounds(const int8_t *k_pool, const float *k
         }
     }
     __syncthreads();                     // the scratch may still be read for the block's previous page
-    if (tid == 0) { *s_bad = 0; }
-    reinterpret_cast<float4 *>(red[warp][0])[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
-    reinterpret_cast<float4 *>(red[warp][1])[lane] = make_float4(lo[0], lo[1], lo[2], lo[3]);
+    if (tid == 0) { sm.bad = 0; }
+    reinterpret_cast<float4 *>(sm.red[warp][0])[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+    reinterpret_cast<float4 *>(sm.red[warp][1])[lane] = make_float4(lo[0], lo[1], lo[2], lo[3]);
     __syncthreads();
-    if (bad) *s_bad = 1;
+    if (bad) sm.bad = 1;
     const int side = tid >> 7, d = tid & 127;                         // threads 0..127: hi, 128..255: lo
-    float b = red[0][side][d];
+    float b = sm.red[0][side][d];
 #pragma unroll
-    for (int k = 1; k < PB_THREADS / 32; ++k) b = side ? fminf(b, red[k][side][d]) : fmaxf(b, red[k][side][d]);
+    for (int k = 1; k < PB_THREADS / 32; ++k) b = side ? fminf(b, sm.red[k][side][d]) : fmaxf(b, sm.red[k][side][d]);
     const float wa = warp_absmax(b);
-    if (lane == 0) s_amax[warp] = wa;
+    if (lane == 0) sm.amax[warp] = wa;
     __syncthreads();
-    float amax = s_amax[0];
+    float amax = sm.amax[0];
 #pragma unroll
-    for (int k = 1; k < PB_THREADS / 32; ++k) amax = fmaxf(amax, s_amax[k]);
-    const bool finite = !*s_bad && amax <= 3.402823466e38f;
+    for (int k = 1; k < PB_THREADS / 32; ++k) amax = fmaxf(amax, sm.amax[k]);
+    const bool finite = !sm.bad && amax <= 3.402823466e38f;
     float t = __fdiv_rn(amax, 127.0f);
     if (t == 0.0f) t = 1.0f;
     const float q = __fdiv_rn(b, t);
     const int code = !finite ? 0 : side ? max(-127, __float2int_rd(q)) : min(127, __float2int_ru(q));
     kb_pool[unit * 2 * PR_HD + tid] = (int8_t)code;
     if (tid == 0) kbs_pool[unit] = finite ? t : CUDART_INF_F;
+}
+
+// A decode step's rows (at most OWN_ROWS), and the bounds of the pages they complete, in one launch: a block takes every row of a
+// head, so all that a completed page holds of this call was written by the block itself.  64 rows x 16 heads: 3.2 us as two
+// launches (and 2 us more of host time).
+constexpr int OWN_ROWS = 256;
+template <typename SrcT, bool VEC>
+__global__ void __launch_bounds__(PR_WARPS * 32) append_head_i8_kernel(const __grid_constant__ PagedRowsArgs a, int8_t *kb_pool, float *kbs_pool) {
+    __shared__ BoundsScratch sm;
+    __shared__ int s_pages[OWN_ROWS], s_n;
+    const int h = blockIdx.x, kv = blockIdx.y;
+    if (threadIdx.x == 0) s_n = 0;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int slot = (int)threadIdx.x < a.n_rows ? a.slot_map[threadIdx.x] : -1;
+#pragma unroll 1
+    for (int r0 = 0; r0 < a.n_rows; r0 += 4 * PR_WARPS) append_rows<SrcT, VEC, 2>(a, kv, h, r0 + (threadIdx.x >> 4), 2 * PR_WARPS);
+    if (kv) return;
+    __syncthreads();                     // the block's codes and scales are in
+    if (slot >= 0 && (unsigned)slot < a.n_slots && slot % PR_PAGE == PR_PAGE - 1) s_pages[atomicAdd(&s_n, 1)] = slot / PR_PAGE;
+    __syncthreads();
+    const int n = s_n;
+    for (int k = 0; k < n; ++k) page_bounds(a.k_pool, a.ks_pool, kb_pool, kbs_pool, (size_t)s_pages[k] * a.nkv + h, sm);
 }
 
 struct PageBoundsArgs {
@@ -180,9 +214,7 @@ struct PageBoundsArgs {
 
 // grid (entry spans, KV heads): a block finds the pages of its span and works them out one after the other.
 __global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_constant__ PageBoundsArgs a) {
-    __shared__ __align__(16) float red[PB_THREADS / 32][2][PR_HD];
-    __shared__ float s_amax[PB_THREADS / 32];
-    __shared__ int s_bad;
+    __shared__ BoundsScratch sm;
     __shared__ int s_pages[PB_THREADS], s_n;
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
@@ -202,7 +234,7 @@ __global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_co
     __syncthreads();
     const int n = s_n;
     for (int k = 0; k < n; ++k)
-        page_bounds(a.k_pool, a.ks_pool, a.kb_pool, a.kbs_pool, (size_t)s_pages[k] * a.nkv + blockIdx.y, red, s_amax, &s_bad);
+        page_bounds(a.k_pool, a.ks_pool, a.kb_pool, a.kbs_pool, (size_t)s_pages[k] * a.nkv + blockIdx.y, sm);
 }
 
 static int launch_bounds(cudaStream_t st, const PageBoundsArgs &in, const char *who) {
@@ -240,6 +272,16 @@ int launch_append_slots_i8(cudaStream_t st, const void *src_k, const void *src_v
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
+    if (kb_pool != nullptr && n_rows <= OWN_ROWS) {
+        cfg.gridDim = dim3(nkv, 2); cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
+        cfg.attrs = pdl; cfg.numAttrs = 1;
+        void (*kernel)(PagedRowsArgs, int8_t *, float *) = src_bf16 ? (vec ? append_head_i8_kernel<__nv_bfloat16, true> : append_head_i8_kernel<__nv_bfloat16, false>)
+                                                                    : (vec ? append_head_i8_kernel<float, true> : append_head_i8_kernel<float, false>);
+        cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, static_cast<int8_t *>(kb_pool), static_cast<float *>(kbs_pool));
+        if (e == cudaSuccess) e = cudaGetLastError();
+        if (e != cudaSuccess) { set_error("%s: %s", who, cudaGetErrorString(e)); return NOMOS_ECUDA; }
+        return NOMOS_OK;
+    }
     const int per_block = ((2 * PR_WARPS) >> a.head_bits) * (many ? 2 : 1);
     cfg.gridDim = dim3((unsigned)(((long)n_rows + per_block - 1) / per_block), 2, (nkv + 2 * PR_WARPS - 1) / (2 * PR_WARPS));
     cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;

@@ -40,6 +40,21 @@ def _addr(x) -> int:
     return x.data_ptr()            # torch tensor
 
 
+_DATA_PTR = None
+
+
+def _addrs(*xs) -> list:
+    """``_addr`` of each: in one go where all are tensors, which is most of the time."""
+    global _DATA_PTR
+    if _DATA_PTR is None:
+        import torch
+        _DATA_PTR = torch.Tensor.data_ptr
+    try:
+        return list(map(_DATA_PTR, xs))
+    except TypeError:
+        return [_addr(x) for x in xs]
+
+
 def _stream(stream) -> C.c_void_p:
     if stream is None:
         return C.c_void_p(_current_stream())
@@ -340,9 +355,8 @@ def kv_paged_plan(stream, seq_lens, n_new, held, free_pages, free_count, block_t
     """Block tables and slot maps of a step from request lengths, all int32 on the GPU; see include/nomos_attn.h.
     ``n_new`` < 0 hands a finished request's pages back; ``granted`` tells which requests got their pages."""
     _check(_lib.lib().nomos_kv_paged_plan(_stream(stream), _PLAN.pack(
-        _PLAN.size, _addr(seq_lens), _addr(n_new), _addr(held), _addr(free_pages), _addr(free_count), _addr(block_table), _addr(held_out),
-        _addr(free_count_out), _addr(granted), _addr(row_start), _addr(slot_map), _addr(row_seq), _addr(row_pos), batch, max_pages, n_pages,
-        max_rows)))
+        _PLAN.size, *_addrs(seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start, slot_map,
+                            row_seq, row_pos), batch, max_pages, n_pages, max_rows)))
 
 
 def kv_paged_append_rows_i8(stream, src_k, src_v, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, slot_map, *, n_rows, nkv, l_hd, l_kvd,
@@ -350,8 +364,7 @@ def kv_paged_append_rows_i8(stream, src_k, src_v, k_pool, v_pool, ks_pool, vs_po
     """Quantising append of any number of rows by slot map; with ``kb_pool`` / ``kbs_pool`` (else ``None``) also the bounds of
     every page whose last row is among them."""
     _check(_lib.lib().nomos_kv_paged_append_rows_i8(_stream(stream), _ROWS.pack(
-        _ROWS.size, _addr(src_k), _addr(src_v), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool), _addr(kbs_pool),
-        _addr(slot_map), n_rows, nkv, l_hd, l_kvd, n_pages, src_type)))
+        _ROWS.size, *_addrs(src_k, src_v, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, slot_map), n_rows, nkv, l_hd, l_kvd, n_pages, src_type)))
 
 
 def kv_paged_page_bounds_i8(stream, k_pool, ks_pool, kb_pool, kbs_pool, pages, *, n, nkv, l_hd, n_pages):
@@ -373,8 +386,8 @@ def attn_paged_sparse_i8(stream, q, k_pool, v_pool, ks_pool, vs_pool, kb_pool, k
     """Attention of ``rows`` query rows (decode, verify and prompt rows alike: sequence ``row_seq[r]``, position ``row_pos[r]``)
     over at most ``top_pages`` pages each, selected per row and KV head by a bound on the logits; see include/nomos_attn.h."""
     _check(_lib.lib().nomos_attn_paged_sparse_i8(_stream(stream), _SPARSE.pack(
-        _SPARSE.size, _addr(q), _addr(k_pool), _addr(v_pool), _addr(ks_pool), _addr(vs_pool), _addr(kb_pool), _addr(kbs_pool), _addr(block_table),
-        _addr(row_seq), _addr(row_pos), _addr(out), _addr(sel_pages), _addr(workspace), int(ws_bytes), rows, batch, nh, nkv, kvg, l_hd, n_pages,
+        _SPARSE.size, *_addrs(q, k_pool, v_pool, ks_pool, vs_pool, kb_pool, kbs_pool, block_table, row_seq, row_pos, out, sel_pages, workspace),
+        int(ws_bytes), rows, batch, nh, nkv, kvg, l_hd, n_pages,
         max_pages, max_len, top_pages, sink_pages, local_pages, softmax_scale, q_type, out_type)))
 
 
@@ -383,8 +396,8 @@ def spec_verify(stream, target_probs, draft_probs, draft_tokens, n_draft, u_acce
     """Speculative verification from given random numbers: accepted drafts, and the next token from the residual (or, all
     accepted, from the target's last row); see include/nomos_attn.h.  ``draft_probs``, ``n_draft``, ``seq_lens`` may be ``None``."""
     _check(_lib.lib().nomos_attn_spec_verify(_stream(stream), _VERIFY.pack(
-        _VERIFY.size, _addr(target_probs), _addr(draft_probs), _addr(draft_tokens), _addr(n_draft), _addr(u_accept), _addr(u_sample),
-        _addr(seq_lens), _addr(seq_lens_out), _addr(n_accepted), _addr(out_tokens), batch, max_draft, vocab, p_stride, q_stride)))
+        _VERIFY.size, *_addrs(target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens),
+        batch, max_draft, vocab, p_stride, q_stride)))
 
 
 class KvRing:
