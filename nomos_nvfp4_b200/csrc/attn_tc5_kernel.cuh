@@ -392,6 +392,9 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
         // a list of pages per sequence, or (unit_lists) per query row and KV head
         const size_t tb = p.unit_lists ? (size_t)b * p.nkv + kvh : (size_t)b;
         const int len = p.seq_lens[tb];
+        // every page of the split is looked up without waiting for the length (what lies behind it is not used)
+        for (int i = threadIdx.x; i < min(p.tiles_per_split, p.max_pages - tile_begin); i += NTHREADS)
+            page_ids[i] = p.block_table[tb * p.max_pages + tile_begin + i];
         if (p.unit_lists && len <= 0) {                  // a row that is skipped: its output stays as it is
             tc_fence_before();
             __syncthreads();
@@ -402,7 +405,6 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
         wg.n_a = (len + KT - 1) / KT;
         tile_end = min(wg.n_a, tile_begin + p.tiles_per_split);
         my_n = max(0, tile_end - tile_begin);
-        for (int i = threadIdx.x; i < my_n; i += NTHREADS) page_ids[i] = p.block_table[tb * p.max_pages + tile_begin + i];
         __syncthreads();
     }
 
