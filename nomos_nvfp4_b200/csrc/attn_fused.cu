@@ -585,12 +585,16 @@ static Tc5Plan tc5_plan(const AttnArgs &a, int ns, int occupancy) {
             const long fixed = 16 + 16L * units;
             max_splits = (int)std::max<long>(1, std::min<long>(max_splits, a.workspace ? (a.ws_bytes - fixed) / per_split : 0));
         }
-        struct Memo { int ntiles, units, slots_gpu, max_splits, best; };          // (as in make_plan: the last few answers, per thread)
+        struct Memo { int ntiles, units, slots_gpu, max_splits, merge_rows, best; };          // (as in make_plan: the last few answers, per thread)
         static thread_local Memo memo[4] = {};
         static thread_local int memo_next = 0;
         bool hit = false;
+        // Selected pages: few tiles per unit, so that the merge shows.  One row of 524288 keys, 8 KV heads x 4 rows, 64 pages: 26.7 /
+        // 25.0 / 26.1 / 32.3 us with 8 / 16 / 32 / 64 splits; 4 heads x 2 rows, 16 pages: 13.3 / 11.7 / 11.7 with 4 / 8 / 16.
+        const int merge_rows = a.unit_lists ? slots : 0;
+        const double per_split = a.unit_lists ? 0.05 * slots : 0.03;
         for (const Memo &m : memo)
-            if (m.best > 0 && m.ntiles == pl.ntiles && m.units == units && m.slots_gpu == slots_gpu && m.max_splits == max_splits) { best = m.best; hit = true; break; }
+            if (m.best > 0 && m.ntiles == pl.ntiles && m.units == units && m.slots_gpu == slots_gpu && m.max_splits == max_splits && m.merge_rows == merge_rows) { best = m.best; hit = true; break; }
         for (int n = 1; !hit && n <= max_splits; ++n) {
             const int tps = (pl.ntiles + n - 1) / n;
             if ((pl.ntiles + tps - 1) / tps != n) continue;
@@ -598,10 +602,10 @@ static Tc5Plan tc5_plan(const AttnArgs &a, int ns, int occupancy) {
             const long waves = (ctas + slots_gpu - 1) / slots_gpu;
             // in units of one tile's streaming time per CTA: a wave costs its tiles plus ~3 of start-up
             // and drain; more than one split adds the partial store, arrival and merge at the end
-            const double cost = (double)waves * (tps + 3.0) + (n > 1 ? 3.0 + 0.03 * n : 0.0);
+            const double cost = (double)waves * (tps + 3.0) + (n > 1 ? 3.0 + per_split * n : 0.0);
             if (cost < best_cost) { best_cost = cost; best = n; }
         }
-        if (!hit) { memo[memo_next] = Memo{pl.ntiles, units, slots_gpu, max_splits, best}; memo_next = (memo_next + 1) % 4; }
+        if (!hit) { memo[memo_next] = Memo{pl.ntiles, units, slots_gpu, max_splits, merge_rows, best}; memo_next = (memo_next + 1) % 4; }
     }
     if (paged && (pl.ntiles + best - 1) / best > tc5::MAX_PAGED_TILES) best = (pl.ntiles + tc5::MAX_PAGED_TILES - 1) / tc5::MAX_PAGED_TILES;
     pl.tiles_per_split = (pl.ntiles + best - 1) / best;
