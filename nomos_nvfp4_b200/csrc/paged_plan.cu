@@ -3,9 +3,9 @@
 //   need_b  = pages request b lacks for len_b + n_b keys, 0 where it cannot be served
 //   upto_b  = sum of need up to and including b: granted while upto_b fits the free pages (finished requests' included)
 // A few thousand requests are three prefix sums; what costs is the latency of one launch and the 12 bytes written per row.
-// So every CTA of one thread-block cluster works the sums out for itself in shared memory (no global scratch, no second
-// launch) and the CTAs share the rows.  held_out may be held itself and free_count_out free_count: the cluster meets once
-// between the last read of the inputs and the first write.
+// So every CTA works the sums out for itself in shared memory (no global scratch, no second launch) and the CTAs share the
+// rows.  Where an output is an input's array (held_out = held, free_count_out = free_count: one step after another), the
+// CTAs are one thread-block cluster that meets once between the last read of the inputs and the first write.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -25,6 +25,7 @@ struct PlanParams {
     int *block_table, *held_out, *free_count_out, *granted, *row_start, *slot_map, *row_seq, *row_pos;
     int batch, max_pages, n_pages, max_rows;
     int vec;                             // the three row arrays start on 16-byte boundaries
+    int in_place;                        // an output lies over an input: the grid is one cluster
 };
 
 struct Sums { long long rows, need, rel; };
@@ -125,8 +126,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
         s_rel[b] = (int)min(rel, 0x7fffffffll);
     }
     if (taken > 0) atomicMax(&s_taken, taken);
-    // everything that may be overwritten in place has been read: the cluster's CTAs may write from here on
-    if (gridDim.x > 1) cluster.sync();
+    // everything that may be overwritten in place has been read: the CTAs may write from here on
+    if (p.in_place && gridDim.x > 1) cluster.sync();
     else __syncthreads();
     const int T = s_taken;
 
@@ -187,11 +188,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const __grid_c
     }
     // the new pages' table entries, and the released pages back onto the stack.  (No CTA reads a table entry or a stack
     // entry that another one writes: new entries lie behind the held ones, pushes at or above F.)
-    for (int e = tid; e < T; e += nthreads) {
+    // (the first CTA has the requests' own numbers to write: these start at the last one and in the middle)
+    for (int e = nthreads - 1 - tid; e < T; e += nthreads) {
         const int b = first_above(s_upto, B, e), i = e - need_before(b);
         p.block_table[(size_t)b * p.max_pages + s_held[b] + i] = stack(top - e);
     }
-    for (int e = tid; e < R; e += nthreads)
+    for (int e = tid >= nthreads / 2 ? tid - nthreads / 2 : tid + (nthreads + 1) / 2; e < R; e += nthreads)
         if (F + e < p.n_pages) p.free_pages[F + e] = released(e);
     if (blockIdx.x == 0) {
         for (int b = threadIdx.x; b < B; b += blockDim.x) {
@@ -212,15 +214,25 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
                       int *block_table, int *held_out, int *free_count_out, int *granted, int *row_start, int *slot_map, int *row_seq,
                       int *row_pos, int batch, int max_pages, int n_pages, int max_rows) {
     PlanParams p{seq_lens, n_new, held, free_pages, free_count, block_table, held_out, free_count_out, granted, row_start, slot_map,
-                 row_seq, row_pos, batch, max_pages, n_pages, max_rows, 0};
+                 row_seq, row_pos, batch, max_pages, n_pages, max_rows, 0, 0};
     p.vec = ((reinterpret_cast<uintptr_t>(slot_map) | reinterpret_cast<uintptr_t>(row_seq) | reinterpret_cast<uintptr_t>(row_pos)) & 15) == 0;
     const size_t smem = (size_t)batch * 5 * sizeof(int);
     cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_MAX_BATCH * 5 * (int)sizeof(int)) : cudaSuccess;
     if (e != cudaSuccess) { set_error("nomos_kv_paged_plan: shared memory: %s", cudaGetErrorString(e)); return NOMOS_ECUDA; }
-    // One CTA while its threads cover the rows in one round; else a cluster of sixteen CTAs of half the threads, eight where the
-    // driver does not allow that: the sums are every CTA's own work, the rows are shared.
-    int ctas = max_rows <= 4 * PLAN_THREADS ? 1 : 16;
-    if (ctas == 16 && cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    const auto over = [](const void *x, long nx, const void *y, long ny) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+        return a < b + 4 * (uintptr_t)ny && b < a + 4 * (uintptr_t)nx;
+    };
+    const struct { const void *x; long n; } ins[4] = {{seq_lens, batch}, {n_new, batch}, {held, batch}, {free_count, 1}},
+                                            outs[7] = {{held_out, batch}, {free_count_out, 1}, {granted, batch}, {row_start, batch + 1l},
+                                                       {slot_map, max_rows}, {row_seq, max_rows}, {row_pos, max_rows}};
+    for (const auto &o : outs)
+        for (const auto &in : ins) p.in_place |= over(o.x, o.n, in.x, in.n) ? 1 : 0;
+    // One CTA while its threads cover the rows in one round.  Else CTAs of half the threads, enough to cover them in one round,
+    // at most one per SM; in place a cluster of sixteen, of eight where the driver does not allow that.  261120 rows of 1024
+    // requests: 7.4 us with 128 CTAs of 512 threads (8.9 with 64 of 1024, 9.1 with 148 of 256), 21.3 in a cluster of sixteen.
+    int ctas = max_rows <= 4 * PLAN_THREADS ? 1 : p.in_place ? 16 : std::min(148, (max_rows + 2 * PLAN_THREADS - 1) / (2 * PLAN_THREADS));
+    if (p.in_place && ctas == 16 && cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
         ctas = 8;
     }
@@ -229,13 +241,13 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = p.in_place ? ctas : 1; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(ctas > 1 ? PLAN_THREADS / 2 : std::min(PLAN_THREADS, (most + 31) / 32 * 32));
     cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, paged_plan_kernel, p);
-    if (e != cudaSuccess && ctas == 16) {
+    if (e != cudaSuccess && p.in_place && ctas == 16) {
         cudaGetLastError();
         cfg.gridDim = dim3(8);
         attr[1].val.clusterDim.x = 8;
