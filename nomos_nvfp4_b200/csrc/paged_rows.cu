@@ -140,17 +140,18 @@ __device__ __forceinline__ void page_bounds(const int8_t *k_pool, const float *k
     float hi[4], lo[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) { hi[e] = -CUDART_INF_F; lo[e] = CUDART_INF_F; }
+    // two rows at a time: the largest and the smallest of three are one instruction each
 #pragma unroll
-    for (int i = 0; i < RPW; ++i) {
-        const float s = __shfl_sync(0xffffffffu, sc, i);
-        const uint32_t w = raw[i] ^ 0x80808080u;
+    for (int i = 0; i < RPW; i += 2) {
+        const float s0 = __shfl_sync(0xffffffffu, sc, i), s1 = __shfl_sync(0xffffffffu, sc, i + 1);
+        const uint32_t u0 = raw[i] ^ 0x80808080u, u1 = raw[i + 1] ^ 0x80808080u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             // code + 128 as the low byte of the float 2^23 + code + 128: no conversion instruction (a quarter of the rate)
-            const float c = __uint_as_float(prmt(w, 0x4b000000u, 0x7440u | e)) - 8388736.0f;
-            const float v = __fmul_rn(c, s);
-            hi[e] = fmaxf(hi[e], v);
-            lo[e] = fminf(lo[e], v);
+            const float v0 = __fmul_rn(__uint_as_float(prmt(u0, 0x4b000000u, 0x7440u | e)) - 8388736.0f, s0);
+            const float v1 = __fmul_rn(__uint_as_float(prmt(u1, 0x4b000000u, 0x7440u | e)) - 8388736.0f, s1);
+            hi[e] = fmaxf(hi[e], fmaxf(v0, v1));
+            lo[e] = fminf(lo[e], fminf(v0, v1));
         }
     }
     __syncthreads();                     // the scratch may still be read for the block's previous page
