@@ -466,7 +466,7 @@ typedef struct nomos_kv_plan {
 int32_t nomos_kv_paged_plan(void *stream, const nomos_kv_plan_t *args);
 /* Quantising append of n_rows rows (src [n_rows][nkv][l_hd] of src_type, row stride l_kvd elements) into slots slot_map[r] of
  * the pools, with the row codec of nomos_kv_append_quant_i8.  Slots outside the pool (-1: padding) are skipped; a slot may
- * occur once.  With kb_pool and kbs_pool (else both 0) the bounds of each page whose row 127 is among the slots are computed
+ * occur once; at most 2^30 rows of single heads per call.  With kb_pool and kbs_pool (else both 0) the bounds of each page whose row 127 is among the slots are computed
  * once all rows are in: kb_pool [n_pages][nkv][2][128] int8 (16-byte aligned), kbs_pool [n_pages][nkv] fp32.  With v the page's
  * dequantised keys, per channel the largest and the smallest, divided by t = (largest magnitude) / 127 and rounded up and
  * down: t * kb[0] >= v >= t * kb[1] up to one rounding.  A page with a row scale that is not finite gets t = +inf, codes 0. */

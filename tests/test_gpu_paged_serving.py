@@ -161,6 +161,42 @@ def test_append_rows(dtype, nkv, gap, shift):
     assert (host(kb)[rest] == 99).all() and (host(kbs)[rest] == 77).all(), "bounds of pages that are not complete"
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("nkv,rows,gap,shift", [(1, 1, 0, 0), (2, 256, 8, 0), (17, 130, 0, 0), (40, 64, 3, 1), (5, 257, 0, 0), (33, 700, 0, 2), (8, 3000, 16, 0)])
+def test_append_rows_up_to_page_ends(dtype, nkv, rows, gap, shift):
+    """Few rows (one launch, a block per head) and many (two launches), head counts on both sides of a block's sixteen, pages completed over
+    two calls, and untouched elsewhere."""
+    rng = np.random.default_rng(nkv * 7 + rows)
+    n_pages = rows // PAGE + 5
+    pages = rng.permutation(n_pages)
+    base = 100                                                         # the first call leaves pages at 100, 228, ... of the sequence
+    pos = np.concatenate([np.arange(base), base + np.arange(rows)])
+    slots = pages[pos // PAGE] * PAGE + pos % PAGE
+    width = nkv * HD + gap
+    pools = empty_pools(n_pages, nkv, 3)
+    codes, scales = np.full((n_pages, nkv, PAGE, HD), 3, np.int8), np.full((n_pages, nkv, PAGE), 2, np.float32)
+    done = set()
+    for part in (slice(0, base), slice(base, base + rows)):
+        n = len(pos[part])
+        flat = torch.from_numpy(rng.standard_normal(n * width + shift, dtype=np.float32)).to(DEV)
+        flat = flat.to(torch.bfloat16) if dtype == "bf16" else flat
+        x = flat[shift:].float().cpu().numpy().reshape(n, width)[:, :nkv * HD].reshape(n, nkv, HD)
+        ops.kv_paged_append_rows_i8(None, flat[shift:], flat[shift:], *pools, i32(slots[part]), n_rows=n, nkv=nkv, l_hd=HD, l_kvd=width, n_pages=n_pages,
+                                    src_type=ops.BF16 if dtype == "bf16" else ops.F32)
+        torch.cuda.synchronize()
+        c, s = ref.codec(x)
+        codes[slots[part] // PAGE, :, slots[part] % PAGE], scales[slots[part] // PAGE, :, slots[part] % PAGE] = c, s
+        done |= {int(p) // PAGE for p in slots[part] if p % PAGE == PAGE - 1}
+        for i in (0, 1):
+            assert np.array_equal(host(pools[i]), codes) and np.array_equal(host(pools[2 + i]), scales)
+        kb, kbs = ref.bounds(codes, scales)
+        for p in range(n_pages):
+            if p in done:
+                assert np.array_equal(host(pools[4])[p], kb[p]) and np.array_equal(host(pools[5])[p], kbs[p]), p
+            else:
+                assert (host(pools[4])[p] == 99).all() and (host(pools[5])[p] == 77).all(), p
+
+
 def test_append_rows_is_the_one_row_append():
     """The same codes and scales as the decode append, rows with infinities, NaN, zeros and denormals among them; no bounds asked for."""
     rng = np.random.default_rng(3)
@@ -452,6 +488,46 @@ def test_verify_without_drafts():
     rng = np.random.default_rng(1)
     p, _, _, _, us = verify_case(rng, 4, 0, 777)
     run_verify(p, None, np.zeros((4, 0), np.int32), None, np.zeros((4, 0), np.float32), us, lens=[0, 1, 2, 3])
+
+
+def test_verify_more_sequences_than_a_grid():
+    """65535 sequences make a launch."""
+    rng = np.random.default_rng(6)
+    batch, k, vocab = 65535 + 9, 1, 3
+    p = rng.dirichlet(np.ones(vocab), (batch, k + 1)).astype(np.float32)
+    q = rng.dirichlet(np.ones(vocab), (batch, k)).astype(np.float32)
+    run_verify(p, q, rng.integers(0, vocab, (batch, k)), rng.integers(-1, k + 1, batch), rng.random((batch, k), dtype=np.float32), rng.random(batch, dtype=np.float32),
+               lens=rng.integers(0, 9, batch))
+
+
+def test_operators_on_two_streams_at_once():
+    """The whole-number operators hold no state between calls: two of each in flight on two streams."""
+    rng = np.random.default_rng(13)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    cases = [plan_case(rng, 700 + i, 6, 90, 20, False) for i in range(2)]
+    probs = [verify_case(rng, 3, 4, 3000 + i) for i in range(2)]
+    work = []
+    for i, c in enumerate(cases):
+        lens, n_new, held, free, count, table = c
+        max_rows = int(np.maximum(n_new, 0).sum())
+        d = {"lens": i32(lens), "n_new": i32(n_new), "held": i32(held), "free": i32(free), "count": i32([count]), "table": i32(table),
+             "held_out": i32(held * 0), "free_count_out": i32([0]), "granted": i32(held * 0), "row_start": i32(np.zeros(len(lens) + 1))}
+        d |= {n: i32(np.zeros(max_rows)) for n in ("slot_map", "row_seq", "row_pos")}
+        p, q, tokens, ua, us = probs[i]
+        v = [dev(p), dev(q), i32(tokens), None, dev(ua), dev(us), None, None, i32(np.zeros(3)), i32(np.zeros((3, 5)))]
+        work.append((d, v, max_rows))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (d, v, max_rows) in enumerate(work):
+            ops.kv_paged_plan(streams[i], d["lens"], d["n_new"], d["held"], d["free"], d["count"], d["table"], d["held_out"], d["free_count_out"], d["granted"],
+                              d["row_start"], d["slot_map"], d["row_seq"], d["row_pos"], batch=700 + i, max_pages=6, n_pages=len(cases[i][3]), max_rows=max_rows)
+            ops.spec_verify(streams[i], *v, batch=3, max_draft=4, vocab=3000 + i, p_stride=3000 + i, q_stride=3000 + i)
+    torch.cuda.synchronize()
+    for i, (d, v, max_rows) in enumerate(work):
+        same_plan(d, ref.plan(*cases[i], max_rows))
+        p, q, tokens, ua, us = probs[i]
+        for b, w in enumerate(ref.verify(p, q, tokens, None, ua, us)):
+            assert (int(v[8][b]), v[9][b].tolist()) == w
 
 
 def test_verify_corners():
