@@ -99,20 +99,27 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 1) paged_select_kernel(const _
             x.t_page[k] = p.kbs_pool[u];
         }
     };
+    float xq[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const size_t at = ((size_t)row * p.nh + h * p.kvg + min(warp + nwarps * i, p.kvg - 1)) * SEL_HD + lane;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            xq[i][k] = p.q_bf16 ? __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(p.q) + at + 32 * k) << 16)
+                                : __ldcg(reinterpret_cast<const float *>(p.q) + at + 32 * k);
+    }
     PageStep cur;
     int s = rank * nwarps + warp;
     if (s < steps) load_step(s, cur);
     // ---- the group's queries, a warp per head
-    for (int j = warp; j < 8; j += nwarps) {
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (j < p.kvg) {
-            const size_t at = ((size_t)row * p.nh + h * p.kvg + j) * SEL_HD + lane;
+    for (int i2 = 0; i2 < 2; ++i2) {
+        const int j = warp + nwarps * i2;
+        if (j >= 8) break;
+        float x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float v = p.q_bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p.q)[at + 32 * k] << 16)
-                                         : reinterpret_cast<const float *>(p.q)[at + 32 * k];
-                x[k] = fabsf(v) <= SEL_FLT_MAX ? v : 0.0f;
-            }
+        for (int k = 0; k < 4; ++k) {
+            x[k] = i2 ? xq[1][k] : xq[0][k];
+            x[k] = fabsf(x[k]) <= SEL_FLT_MAX ? x[k] : 0.0f;
         }
         const float amax = warp_absmax(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
         float scale = __fdiv_rn(amax, 127.0f);
