@@ -824,6 +824,9 @@ NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_s
         a.q = s.q; a.k_cache = ptr(c->k_pool); a.v_cache = ptr(c->v_pool); a.k_scales = ptr(c->ks_pool); a.v_scales = ptr(c->vs_pool);
         a.out = ptr(c->out + (uint64_t)r0 * nh * l_hd * os);
         a.block_table = s.lists; a.seq_lens = s.lens;
+        // as many rows for each sequence as there is room for, the rest padding: exact for decode and verify steps padded to a
+        // captured size, and nothing but the split depends on it
+        a.live_rows = nr > c->batch ? nr / (int)c->batch * (int)c->batch : 0;
         a.workspace = ptr(c->workspace + w.lists + w.lens); a.ws_bytes = w.attn;
         a.softmax_scale = (float)c->softmax_scale; a.q_type = (int)c->q_type; a.out_type = (int)c->out_type;
         rc = launch_paged_select(as_stream(stream), s);

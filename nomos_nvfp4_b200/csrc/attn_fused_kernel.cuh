@@ -137,6 +137,7 @@ struct KParams {
     long q_batch_stride, kv_batch_stride, scale_batch_stride, out_batch_stride;
     const int *block_table;  // paged caches (tcgen05 kernel): [batch][max_pages] page of each 128-key tile; nullptr = contiguous
     const int *seq_lens;     // paged caches: keys of each sequence
+    int whole_units;         // unit_lists: the first so many (query row, KV head) units are not split (their CTAs of split > 0 leave at once)
     int unit_lists;          // paged caches: block_table and seq_lens have a row per (query row, KV head) instead of per sequence
     int max_pages;
     // sequence-sharded decode across GPUs (peer_world > 1): the CTA that merges a unit's splits pushes the unit's

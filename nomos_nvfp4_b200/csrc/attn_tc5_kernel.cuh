@@ -330,8 +330,13 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
     wg.len_a = min(p.klen - wg.tbase, p.cache_cap - wg.ring0);
     wg.a0 = wg.ring0 & ~3;
     wg.n_a = (wg.ring0 + wg.len_a - wg.a0 + KT - 1) / KT;
-    const int tile_begin = split * p.tiles_per_split;
-    int tile_end = min(p.ntiles, tile_begin + p.tiles_per_split);
+    // selected pages: units that fill the GPU in whole rounds are served by one CTA each, the others are split
+    // (paged calls have at most eight slots: the instances with more of them carry none of this)
+    const bool whole = !C::WIDE && b * p.nkv + kvh < p.whole_units;
+    if (whole && split > 0) return;                   // (the grid still ends after its predecessor: other CTAs wait for it)
+    const int tiles_per_split = whole ? p.ntiles : p.tiles_per_split;
+    const int tile_begin = split * tiles_per_split;
+    int tile_end = min(p.ntiles, tile_begin + tiles_per_split);
     int my_n = max(0, tile_end - tile_begin);
     const int row_base = kvh * p.cache_cap;          // this head's first row in the {rows} dimension of the maps
     // Paged caches (block_table != nullptr): the sequence's tile j lives in page block_table[b][j] of the
@@ -390,12 +395,12 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
     }
     if (paged) {
         // a list of pages per sequence, or (unit_lists) per query row and KV head
-        const size_t tb = p.unit_lists ? (size_t)b * p.nkv + kvh : (size_t)b;
+        const size_t tb = !C::WIDE && p.unit_lists ? (size_t)b * p.nkv + kvh : (size_t)b;
         const int len = p.seq_lens[tb];
         // every page of the split is looked up without waiting for the length (what lies behind it is not used)
-        for (int i = threadIdx.x; i < min(p.tiles_per_split, p.max_pages - tile_begin); i += NTHREADS)
+        for (int i = threadIdx.x; i < min(tiles_per_split, p.max_pages - tile_begin); i += NTHREADS)
             page_ids[i] = p.block_table[tb * p.max_pages + tile_begin + i];
-        if (p.unit_lists && len <= 0) {                  // a row that is skipped: its output stays as it is
+        if (!C::WIDE && p.unit_lists && len <= 0) {                  // a row that is skipped: its output stays as it is
             tc_fence_before();
             __syncthreads();
             if (warp == NSW) tmem_dealloc(tmem_base, C::TMEM_COLS);
@@ -403,14 +408,14 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
         }
         wg.klen = len; wg.ring0 = 0; wg.a0 = 0; wg.len_a = len;
         wg.n_a = (len + KT - 1) / KT;
-        tile_end = min(wg.n_a, tile_begin + p.tiles_per_split);
+        tile_end = min(wg.n_a, tile_begin + tiles_per_split);
         my_n = max(0, tile_end - tile_begin);
         __syncthreads();
     }
 
     auto make_tail_args = [&]() {
         TailArgs t;
-        t.partial = p.write_partial ? p.partial + ((size_t)split * p.grows) * (HD + 2) : nullptr;
+        t.partial = p.write_partial && !whole ? p.partial + ((size_t)split * p.grows) * (HD + 2) : nullptr;
         t.out = p.out; t.out_batch_stride = p.out_batch_stride;
         t.export_nat = p.export_nat; t.out_type = p.out_type; t.S = p.S; t.nh = p.nh;
         t.kvg = p.kvg; t.kvg_magic = p.kvg_magic;
@@ -804,7 +809,7 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
             const int idx = rg * NS + s;
             const int r = fused::div_kvg(p, idx);
             const int hrow = r * p.nh + kvh * p.kvg + (idx - r * p.kvg);          // row within the batch element
-            if (p.write_partial) {
+            if (p.write_partial && !whole) {
                 float *pr = pbase + (size_t)(b * p.S * p.nh + hrow) * (HD + 2);
                 pr[0] = a;
                 if (kr == 0) {
@@ -865,7 +870,7 @@ __global__ void __launch_bounds__(Cfg<NS>::NTHREADS, Cfg<NS>::MIN_CTAS)
     tc_fence_before();
     __syncthreads();
     if (warp == NSW) tmem_dealloc(tmem_base, C::TMEM_COLS);
-    fused::merge_splits_in_kernel<NS, HD, NTHREADS, 8>(p, sm, b, kvh, rg);
+    if (!whole) fused::merge_splits_in_kernel<NS, HD, NTHREADS, 8>(p, sm, b, kvh, rg);
 }
 
 }  // namespace tc5

@@ -84,6 +84,7 @@ struct AttnArgs {
     int max_pages, n_pages;
     int unit_lists;         // 1: block_table [batch][nkv][max_pages] and seq_lens [batch][nkv] (pages listed per query row and
                             // KV head; batch counts query rows); a unit of length 0 is skipped, its output left as it is
+    int live_rows;          // unit_lists: how many of the rows are probably not padding (0: all); for the split alone
     // sequence-sharded decode across GPUs (peer_world > 1, see nomos_attn_seq_sharded): every rank's mailbox as mapped
     // in this process, this rank's index, the step number and the wait limit
     void *peer_box[8];

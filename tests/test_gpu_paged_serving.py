@@ -387,6 +387,20 @@ def test_sparse_ties_zeros_and_pages_that_are_not_finite():
     check_sparse(pools, q[2:4], row_seq[2:4], row_pos[2:4], got[2:4], sel[2:4], top=top)
 
 
+@pytest.mark.parametrize("rows,pad,nkv,kvg,top,idle", [(20, 0, 16, 2, 8, 0), (24, 8, 16, 1, 9, 0), (21, 5, 15, 2, 13, 3), (40, 0, 8, 4, 256, 0), (39, 1, 8, 8, 11, 0)])
+def test_sparse_rounds_of_units_and_a_split_rest(rows, pad, nkv, kvg, top, idle):
+    """More (row, KV head) units than run at once: those left over by whole rounds are split, those before them are not; padding behind
+    and between the rows."""
+    rng = np.random.default_rng(rows + nkv)
+    lens = [int(x) for x in rng.integers(1100, 1700, rows)]
+    pools = Pools(rng, lens, nkv)
+    row_seq, row_pos = np.concatenate([np.arange(rows), np.full(pad, -1)]), np.concatenate([np.array(lens) - 1, np.full(pad, -1)])
+    row_seq[rng.permutation(rows)[:idle]] = -1
+    q = bf16_normal(rng, (rows + pad, nkv * kvg, HD))
+    got, sel = run_sparse(pools, q, row_seq, row_pos, top=top, calls=2)
+    check_sparse(pools, q, row_seq, row_pos, got, sel, top=top)
+
+
 def test_sparse_more_rows_than_one_launch():
     """8192 rows make a launch: the rest takes a second one, with a split and a part of the workspace of its own."""
     rng = np.random.default_rng(10)
