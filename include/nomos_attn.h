@@ -456,7 +456,7 @@ int32_t nomos_kv_paged_append_quant_i8(void *stream, uint64_t src_k, uint64_t sr
  * held_out may be held and free_count_out free_count (one step after another, or a captured graph replayed); with arrays of
  * their own a plan can be dropped: the entries it wrote lie behind what held and free_count count.  seq_lens is not written:
  * add what was kept (nomos_attn_spec_verify does), so rows rejected there are planned again, into the pages already held.
- * At most 8192 requests. */
+ * At most 8192 requests and 2^30 rows. */
 typedef struct nomos_kv_plan {
     uint64_t struct_bytes;
     uint64_t seq_lens, n_new, held, free_pages, free_count, block_table;

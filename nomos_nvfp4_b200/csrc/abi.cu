@@ -683,7 +683,7 @@ NOMOS_EXPORT int32_t nomos_kv_paged_plan(void *stream, const nomos_kv_plan_t *a)
                 a->granted && a->row_start, "%s: null pointer", who);
     REQUIRE(fits32({a->batch, a->max_pages, a->n_pages, a->max_rows}), "%s: dimensions are 32-bit numbers", who);
     REQUIRE(a->max_rows >= 0 && (a->max_rows == 0 || (a->slot_map && a->row_seq && a->row_pos)), "%s: null pointer or negative max_rows", who);
-    REQUIRE(a->max_pages > 0 && a->n_pages > 0, "%s: bad max_pages/n_pages", who);
+    REQUIRE(a->max_pages > 0 && a->n_pages > 0 && a->max_rows <= (1l << 30), "%s: bad max_pages/n_pages/max_rows", who);
     for (uint64_t x : {a->seq_lens, a->n_new, a->held, a->free_pages, a->free_count, a->block_table, a->held_out, a->free_count_out, a->granted,
                        a->row_start, a->slot_map, a->row_seq, a->row_pos})
         REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);

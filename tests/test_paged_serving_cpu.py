@@ -49,7 +49,7 @@ def test_plan_refusals(ops):
         refused(ops, -1, ops.kv_paged_plan, 0, *[None if j == i else P for j in range(13)], **kw)
         refused(ops, -1, ops.kv_paged_plan, 0, *[P + 2 if j == i else P for j in range(13)], **kw)
     for bad in (dict(max_pages=0), dict(n_pages=0), dict(max_rows=-1), dict(max_pages=1 << 24), dict(n_pages=1 << 24), dict(batch=1 << 32),
-                dict(max_rows=1 << 31)):
+                dict(max_rows=1 << 31), dict(max_rows=(1 << 30) + 1)):
         refused(ops, -1, ops.kv_paged_plan, 0, *[P] * 13, **{**kw, **bad})
     refused(ops, -2, ops.kv_paged_plan, 0, *[P] * 13, **{**kw, "batch": 8193})
     ops.kv_paged_plan(0, *[None] * 13, **{**kw, "batch": 0})
