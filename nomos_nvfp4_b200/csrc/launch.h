@@ -16,6 +16,13 @@ int launch_append_i8(cudaStream_t st, const void *src_k, const void *src_v, void
 int launch_append_paged_i8(cudaStream_t st, const void *src_k, const void *src_v, void *k_pool, void *v_pool, void *ks_pool,
                            void *vs_pool, const int *block_table, const int *positions, int batch, int nkv, int l_hd, int l_kvd,
                            int max_pages);
+// The current device as a bit, for set-up calls that are made once per device (a function attribute costs half a microsecond);
+// 0 beyond 64 devices: made every time.
+inline uint64_t device_bit() {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    return dev >= 0 && dev < 64 ? 1ull << dev : 0;
+}
 // ---- paged_plan.cu
 constexpr int PLAN_MAX_BATCH = 8192;     // requests of one call: their prefix sums live in shared memory
 int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, const int *held, int *free_pages, const int *free_count,

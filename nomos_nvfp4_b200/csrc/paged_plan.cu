@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "launch.h"
@@ -232,9 +233,14 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
     // at most one per SM; in place a cluster of sixteen, of eight where the driver does not allow that.  261120 rows of 1024
     // requests: 7.4 us with 128 CTAs of 512 threads (8.9 with 64 of 1024, 9.1 with 148 of 256), 21.3 in a cluster of sixteen.
     int ctas = max_rows <= 4 * PLAN_THREADS ? 1 : p.in_place ? 16 : std::min(148, (max_rows + 2 * PLAN_THREADS - 1) / (2 * PLAN_THREADS));
-    if (p.in_place && ctas == 16 && cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-        cudaGetLastError();
-        ctas = 8;
+    static std::atomic<uint64_t> large_clusters{0};                   // devices on which the attribute is set
+    if (p.in_place && ctas == 16 && !(large_clusters.load(std::memory_order_relaxed) & device_bit())) {
+        if (cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+            large_clusters.fetch_or(device_bit(), std::memory_order_relaxed);
+        } else {
+            cudaGetLastError();
+            ctas = 8;
+        }
     }
     const int most = std::max(batch, (max_rows + 3) / 4);
     cudaLaunchAttribute attr[2];
@@ -245,7 +251,7 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(ctas > 1 ? PLAN_THREADS / 2 : std::min(PLAN_THREADS, (most + 31) / 32 * 32));
-    cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;
+    cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = p.in_place && ctas > 1 ? 2 : 1;
     e = cudaLaunchKernelEx(&cfg, paged_plan_kernel, p);
     if (e != cudaSuccess && p.in_place && ctas == 16) {
         cudaGetLastError();

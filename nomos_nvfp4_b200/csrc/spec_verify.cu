@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "launch.h"
@@ -236,9 +237,14 @@ int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const in
     // 8 / 16; 96 sequences of 32000: 10.2 with 4, 10.5 with 2.
     int ctas = 16;
     while (ctas > 1 && ((long)ctas * std::min(batch, 65535) > 148 * SV_CTAS_PER_SM || vocab < ctas * SV_WARPS * 128 * SV_UNROLL)) ctas /= 2;
-    if (ctas == 16 && cudaFuncSetAttribute(spec_verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-        cudaGetLastError();
-        ctas = 8;
+    static std::atomic<uint64_t> large_clusters{0};                   // devices on which the attribute is set
+    if (ctas == 16 && !(large_clusters.load(std::memory_order_relaxed) & device_bit())) {
+        if (cudaFuncSetAttribute(spec_verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+            large_clusters.fetch_or(device_bit(), std::memory_order_relaxed);
+        } else {
+            cudaGetLastError();
+            ctas = 8;
+        }
     }
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(SV_THREADS); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;

@@ -55,26 +55,28 @@ def _addrs(*xs) -> list:
         return [_addr(x) for x in xs]
 
 
-def _stream(stream) -> C.c_void_p:
+def _stream(stream) -> int:
     if stream is None:
-        return C.c_void_p(_current_stream())
+        return _current_stream()
     if isinstance(stream, int):
-        return C.c_void_p(stream)
-    return C.c_void_p(stream.cuda_stream)
+        return stream
+    return stream.cuda_stream
 
 
-_RAW_STREAM = None
+_RAW_STREAM = _DEVICE = None
 
 
 def _current_stream() -> int:
     """torch's current stream on the current device.  The stream object that torch.cuda.current_stream() builds costs 3 us, most of
     a small call; where torch offers the bare handle (0.1 us) that is taken."""
-    global _RAW_STREAM
-    import torch
+    global _RAW_STREAM, _DEVICE
     if _RAW_STREAM is None:
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _RAW_STREAM = (lambda: raw(torch.cuda.current_device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
-    return _RAW_STREAM()
+        import torch
+        torch.cuda.current_device()                               # initialises CUDA on the first call of the process
+        raw, device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
+        _DEVICE = device if raw and device else lambda: None
+        _RAW_STREAM = raw if raw and device else lambda _: torch.cuda.current_stream().cuda_stream
+    return _RAW_STREAM(_DEVICE())
 
 
 def _check(status: int) -> None:
