@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 1) paged_select_kernel(const _
     hi = __reduce_max_sync(0xffffffffu, hi);
     if (lane == 0) { s_range[0][warp] = lo; s_range[1][warp] = hi; }
     __syncthreads();
-    for (int k = 0; k < nwarps; ++k) { lo = min(lo, s_range[0][k]); hi = max(hi, s_range[1][k]); }
+    lo = __reduce_min_sync(0xffffffffu, lane < nwarps ? s_range[0][lane] : 0xffffffffu);
+    hi = __reduce_max_sync(0xffffffffu, lane < nwarps ? s_range[1][lane] : 0u);
     // all keys that are not forced agree above `bit`; the forced ones (fewer than top, or all that is wanted) lie above them
     const int bits = lo < hi ? 32 - __clz(lo ^ hi) : 0;
     uint32_t thr = bits == 32 ? 0u : (hi >> bits) << bits;
@@ -245,13 +246,10 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 1) paged_select_kernel(const _
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) s_count[0][warp] = make_uint2(above, equal);
     __syncthreads();
-    int above_all = 0, a0 = 0, e0 = 0;   // of all warps; of the warps before this one
-    for (int k = 0; k < nwarps; ++k) {
-        const uint2 c = s_count[0][k];
-        above_all += (int)c.x;
-        a0 += k < warp ? (int)c.x : 0;
-        e0 += k < warp ? (int)c.y : 0;
-    }
+    const uint2 of_warp = lane < nwarps ? s_count[0][lane] : make_uint2(0, 0);
+    const int above_all = (int)__reduce_add_sync(0xffffffffu, of_warp.x);
+    // of the warps before this one
+    int a0 = (int)__reduce_add_sync(0xffffffffu, lane < warp ? of_warp.x : 0u), e0 = (int)__reduce_add_sync(0xffffffffu, lane < warp ? of_warp.y : 0u);
     const int equal_wanted = p.top - above_all;
     for (int i0 = w0; i0 < w1; i0 += 32) {
         const int i = i0 + lane;

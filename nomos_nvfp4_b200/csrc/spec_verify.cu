@@ -57,6 +57,16 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
     return v;
 }
 
+// Inclusive prefix sums over a warp.
+__device__ __forceinline__ unsigned long long warp_prefix(unsigned long long v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
 // Sum over [i0, i1) by one warp, where p + i0 is a 16-byte boundary: batches of 256 elements, every load of a batch in flight
 // before the first weight.  Q: 0 no drafter row, 1 drafter row on the same boundary, 2 drafter row anywhere.
 template <int Q>
@@ -157,18 +167,15 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
             for (int i = 0; i < lead; ++i) mine += w.at(i);
         if (lane == 0) s_warp[round][warp] = mine;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned long long t = 0;
-            for (int k = 0; k < SV_WARPS; ++k) t += s_warp[round][k];
-            s_total[round] = t;
+        if (warp == 0) {
+            const unsigned long long t = warp_sum(lane < SV_WARPS ? s_warp[round][lane] : 0);
+            if (lane == 0) s_total[round] = t;
         }
         cluster.sync();
-        unsigned long long total = 0, before = 0;
-        for (int k = 0; k < C; ++k) {
-            const unsigned long long t = *cluster.map_shared_rank(&s_total[round], k);
-            before += k < rank ? t : 0;
-            total += t;
-        }
+        // every warp fetches the CTAs' totals, a lane each: one trip through the cluster's shared memory
+        const unsigned long long upto = warp_prefix(lane < C ? *cluster.map_shared_rank(&s_total[round], lane) : 0, lane);
+        const unsigned long long total = __shfl_sync(0xffffffffu, upto, 31);
+        const unsigned long long after = __shfl_sync(0xffffffffu, upto, rank), before = after - s_total[round];
         if (total == 0 && round == 0 && (w.q || w.one >= 0)) {
             // the drafter covers the target everywhere (u outside [0, 1) only): the target's own row decides
             w.q = nullptr; w.one = -1;
@@ -177,10 +184,11 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
         if (total > 0) {
             const long long t0 = (long long)floor(__dmul_rn((double)u_sample, (double)total));
             const unsigned long long T = (unsigned long long)max(0ll, min(t0, (long long)total - 1));
-            if (T >= before && T < before + s_total[round]) {         // uniform over the CTA
-                unsigned long long base = before;
-                int k = 0;
-                while (k < SV_WARPS - 1 && T >= base + s_warp[round][k]) base += s_warp[round][k++];
+            if (T >= before && T < after) {                           // uniform over the CTA
+                // the warp whose stretch holds T
+                const unsigned long long mine_w = lane < SV_WARPS ? s_warp[round][lane] : 0, w_upto = before + warp_prefix(mine_w, lane);
+                const int k = min(SV_WARPS - 1, __popc(__ballot_sync(0xffffffffu, lane < SV_WARPS && T >= w_upto)));
+                unsigned long long base = __shfl_sync(0xffffffffu, w_upto - mine_w, k);
                 // the k-th warp's stretch again, by the whole CTA: `each` neighbouring elements per thread
                 const long u0 = (long)rank * SV_WARPS + k;
                 const int j0 = cut(u0), j1 = u0 == (long)C * SV_WARPS - 1 ? a.vocab : cut(u0 + 1);
@@ -188,15 +196,10 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
                 const int e0 = min(j1, j0 + (int)threadIdx.x * each), e1 = min(j1, e0 + each);
                 unsigned long long s = 0;
                 for (int i = e0; i < e1; ++i) s += w.at(i);
-                unsigned long long incl = s;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += v;
-                }
+                const unsigned long long incl = warp_prefix(s, lane);
                 if (lane == 31) s_scan[warp] = incl;
                 __syncthreads();
-                for (int k2 = 0; k2 < warp; ++k2) base += s_scan[k2];
+                base += warp_sum(lane < warp ? s_scan[lane] : 0);
                 const unsigned long long lo = base + incl - s;
                 if (T >= lo && T < lo + s) {                          // one thread of the cluster
                     unsigned long long c = lo;
