@@ -516,6 +516,7 @@ static bool tc5_eligible(const AttnArgs &a) {
 
 struct Tc5Plan {
     int ns, row_groups, tbase, ntiles, splits, tiles_per_split, grows, whole_units;
+    int uniform_splits;          // what every unit would be split into without whole_units
 };
 
 // Where a launch over selected pages may split the units of its last round only (see tc5_plan), and by how much at most: the
@@ -615,6 +616,7 @@ static Tc5Plan tc5_plan(const AttnArgs &a, int ns, int occupancy) {
     // Selected pages, a few rounds of units: those that fill whole rounds are not split, those left over by as many splits as find
     // room in one more round.  16 KV heads x 32 pages: 24 rows 90.6 -> 81.2 us, 20 rows 83.5 -> 70.4.
     pl.whole_units = 0;
+    pl.uniform_splits = best;
     const int live = a.live_rows > 0 ? a.nkv * a.live_rows : units, tail = live % slots_gpu;
     if (tail_splits_ok(a, pl.ntiles) && live > slots_gpu && tail > 0 && 2 * tail <= slots_gpu && a.force_splits == 0) {
         const int m = std::min(TAIL_SPLITS, slots_gpu / tail), tps = (pl.ntiles + best - 1) / best;
@@ -635,9 +637,9 @@ static int launch_tc5_inst(cudaStream_t st, const AttnArgs &a, bool query_ws, lo
     const long part_bytes = (((long)pl.splits * pl.grows * (a.l_hd + 2) * 4) + 15) / 16 * 16;
     const bool in_kernel_merge = pl.splits > 1 || a.peer_world > 1;
     const long need = in_kernel_merge ? part_bytes + units * 16 : 0;
-    if (query_ws && a.unit_lists) {       // many rows, mostly one split each
-        const long tail = ((long)TAIL_SPLITS * pl.grows * (a.l_hd + 2) * 4 + 15) / 16 * 16 + units * 16;
-        *ws_needed = tail_splits_ok(a, pl.ntiles) ? std::max(need, tail) : need;
+    if (query_ws && a.unit_lists) {       // many rows, mostly one split each; either plan of a call has to fit
+        const long most = std::max({pl.splits, pl.uniform_splits, tail_splits_ok(a, pl.ntiles) ? TAIL_SPLITS : 1});
+        *ws_needed = most > 1 ? (most * pl.grows * (a.l_hd + 2) * 4 + 15) / 16 * 16 + units * 16 : 0;
         return NOMOS_OK;
     }
     if (query_ws) { *ws_needed = part_bytes + units * 16; return NOMOS_OK; }   // also enough for a sequence-sharded call, which merges in the kernel even with one split

@@ -401,6 +401,32 @@ def test_sparse_rounds_of_units_and_a_split_rest(rows, pad, nkv, kvg, top, idle)
     check_sparse(pools, q, row_seq, row_pos, got, sel, top=top)
 
 
+def test_sparse_workspace_fits_whatever_is_padding():
+    """The workspace query knows the rows but not the batch, from which a call guesses how many of them are padding and splits accordingly:
+    no call of a sweep over both is refused.  (All rows are padding: the launches write nothing.)"""
+    rng = np.random.default_rng(14)
+    pools = Pools(rng, [300], 1)
+    bufs = pools.device()
+    for nkv, kvg in ((1, 1), (3, 2), (16, 2), (8, 8)):
+        k, v, ks, vs = (torch.zeros((4, nkv, *x.shape[2:]), dtype=x.dtype, device=DEV) for x in bufs[:4])
+        kb, kbs = torch.zeros((4, nkv, 2, HD), dtype=torch.int8, device=DEV), torch.zeros((4, nkv), device=DEV)
+        for rows in (1, 5, 19, 20, 24, 37, 64, 100, 149, 255, 256, 257):
+            q = torch.zeros((rows, nkv * kvg, HD), device=DEV)
+            out = torch.full_like(q, -31)
+            pad = i32(np.full(rows, -1))
+            for top, keys in ((3, 128 * 64), (8, 128 * 64), (9, 128 * 9), (21, 128 * 200), (64, 128 * 64), (250, 128 * 260)):
+                kw = dict(rows=rows, nh=nkv * kvg, nkv=nkv, kvg=kvg, l_hd=HD, top_pages=top, max_len=keys)
+                wsb = ops.attn_paged_sparse_workspace_bytes(**kw)
+                ws = torch.empty(wsb, dtype=torch.uint8, device=DEV)
+                for batch in sorted({1, 2, 3, rows // 5 + 1, rows // 3 + 1, rows // 2 + 1, max(1, rows - 7), rows, 300}):
+                    table = torch.zeros((batch, keys // PAGE), dtype=torch.int32, device=DEV)
+                    ops.attn_paged_sparse_i8(None, q, k, v, ks, vs, kb, kbs, table, pad, pad, out, None, ws, wsb, **kw, batch=batch, n_pages=4,
+                                             max_pages=keys // PAGE)
+            torch.cuda.synchronize()
+            assert bool((out == -31).all())
+    assert ops.device_faults() == 0
+
+
 def test_sparse_more_rows_than_one_launch():
     """8192 rows make a launch: the rest takes a second one, with a split and a part of the workspace of its own."""
     rng = np.random.default_rng(10)
