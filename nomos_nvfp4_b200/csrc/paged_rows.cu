@@ -4,6 +4,8 @@
 // min(127, ceil(hi / t)) and max(-127, floor(lo / t)): rounded outwards, so that  sum_d max(q hi, q lo) * t  is at least
 // q . k of every key of the page.  A page with a row scale that is not finite gets t = +inf and codes 0.
 // Both are streams: a row is read once and written once, a completed page's K codes are read back once, mostly out of L2.
+// 8168 rows x 16 heads: fp32 rows 25.5 us (6.6 TB/s, the copy rate), bf16 rows 21 us (4.8 TB/s, bound by instruction issue); the bounds
+// of their 1024 pages and heads 10 us (17 MB; latency and the ALU pipe).
 #include <math_constants.h>
 
 #include <algorithm>

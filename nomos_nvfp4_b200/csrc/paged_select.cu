@@ -8,6 +8,8 @@
 // `top` in all, listed in ascending order: of the pages listed only the last, the row's own, is partial.
 // Bytes: 260 per page and KV head, against 33 792 for the page itself.  A unit is spread over a cluster (more CTAs read
 // the bounds at once than there are units); its scores meet in the first CTA's shared memory, which selects.
+// Bound by latency: 4.7 us for 4 units of 64 pages, 10.8 us for 384 units of 256 (25 MB of bounds), 10 us for 8 units of 4096, of
+// which scores 2, key range and rounds 3, the lists 2; launches back to back, the rest dependent loads and the cluster's barriers.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -339,6 +339,26 @@ def test_sparse_rows_of_a_sequence(keys, top):
     check_sparse(pools, q, row_seq, row_pos, got, sel, top=top, local=2)
 
 
+@pytest.mark.parametrize("alike", [False, True])
+@pytest.mark.parametrize("pages,tops", [(2300, (3, 100, 143, 144, 700)), (1040, (5, 65, 300)), (4097, (256, 257))])
+def test_sparse_many_pages(pages, tops, alike):
+    """Contexts of thousands of pages (a few physical ones, listed over and over): selection in clusters of every size, more keys than a lane
+    keeps in registers, and pages with equal bounds in every CTA of a cluster, where the lowest numbers win."""
+    rng = np.random.default_rng(pages)
+    nkv, kvg, few = 2, 2, 40
+    pools = Pools(rng, [few * PAGE], nkv)
+    phys = pools.table[0, :few].copy()
+    keys = pages * PAGE - 45
+    pools.lens, pools.max_pages = [keys, 500 * PAGE], pages
+    pools.table = np.stack([phys[:1].repeat(pages) if alike else rng.choice(phys, pages) for _ in range(2)]).astype(np.int32)
+    row_seq, row_pos = np.array([0, 0, 1]), np.array([keys - 1, keys // 2, 500 * PAGE - 1])
+    q = bf16_normal(rng, (3, nkv * kvg, HD))
+    for top in tops:
+        local = 2 if top > 3 else 1
+        got, sel = run_sparse(pools, q, row_seq, row_pos, top=top, local=local)
+        check_sparse(pools, q, row_seq, row_pos, got, sel, top=top, local=local)
+
+
 def test_sparse_over_all_pages_is_paged_decode():
     """top_pages covering every sequence: dense attention, and the dense entry point's output (each within the bar of the exact one)."""
     rng = np.random.default_rng(8)
