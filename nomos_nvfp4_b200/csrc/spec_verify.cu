@@ -236,10 +236,11 @@ int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const in
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     // As many CTAs per sequence as are resident at once, at most sixteen (eight where the driver does not allow that), and none
-    // without a batch of elements for each of its warps.  One sequence of 262144 tokens: 24.0 / 13.6 / 9.0 / 7.3 us with 2 / 4 /
+    // without a load per lane for each of its warps (sixteen: a whole batch; 16 sequences of 50001 tokens 7.0 us with 8, 8.7 with 16;
+    // one of 32000 5.6 with 4, 5.2 with 8).  One sequence of 262144 tokens: 24.0 / 13.6 / 9.0 / 7.3 us with 2 / 4 /
     // 8 / 16; 96 sequences of 32000: 10.2 with 4, 10.5 with 2.
     int ctas = 16;
-    while (ctas > 1 && ((long)ctas * std::min(batch, 65535) > 148 * SV_CTAS_PER_SM || vocab < ctas * SV_WARPS * 128 * SV_UNROLL)) ctas /= 2;
+    while (ctas > 1 && ((long)ctas * std::min(batch, 65535) > 148 * SV_CTAS_PER_SM || vocab < ctas * SV_WARPS * 128 * (ctas > 8 ? SV_UNROLL : 1))) ctas /= 2;
     static std::atomic<uint64_t> large_clusters{0};                   // devices on which the attribute is set
     if (ctas == 16 && !(large_clusters.load(std::memory_order_relaxed) & device_bit())) {
         if (cudaFuncSetAttribute(spec_verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
