@@ -4,8 +4,8 @@
 // min(127, ceil(hi / t)) and max(-127, floor(lo / t)): rounded outwards, so that  sum_d max(q hi, q lo) * t  is at least
 // q . k of every key of the page.  A page with a row scale that is not finite gets t = +inf and codes 0.
 // Both are streams: a row is read once and written once, a completed page's K codes are read back once, mostly out of L2.
-// 8168 rows x 16 heads: fp32 rows 25.5 us (6.6 TB/s, the copy rate), bf16 rows 21 us (4.8 TB/s, bound by instruction issue); the bounds
-// of their 1024 pages and heads 10 us (17 MB; latency and the ALU pipe).
+// 8168 rows x 16 heads: fp32 rows 26 us (6.4 TB/s, close to the copy rate), bf16 rows 22 us (4.6 TB/s, bound by instruction issue); the bounds
+// of their 1024 pages and heads 10 us alone (17 MB; latency and the ALU pipe), 5 beside the V rows.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -44,32 +44,41 @@ __device__ __forceinline__ uint32_t pack_codes(const float *x, float inv) {
     return w;
 }
 
+__device__ __forceinline__ float load_cg(const float *p) { return __ldcg(p); }
+__device__ __forceinline__ float load_cg(const __nv_bfloat16 *p) {
+    return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16);
+}
+
 // Half a warp per row of one (K or V, KV head): lane l holds elements 8l .. 8l + 7, one or two wide loads and one 8-byte store of
 // codes.  The half warp takes rows r0, r0 + rows_step, ... (STEPS of them, loaded before the first use).
 // VEC: rows start on a boundary of eight elements; otherwise the same elements one by one.
+// Everything is read through L2 (ld.global.cg): nothing is read twice, and the V rows of a long append are read in a grid that
+// does not itself wait for their producer (append_v_bounds_i8_kernel).
 template <typename SrcT, bool VEC, int STEPS>
 __device__ __forceinline__ void append_rows(const PagedRowsArgs &a, int kv, int h, int r0, int rows_step) {
+    // wide fp32 loads: lane l holds elements 4l .. 4l + 3 of each half of the row, so that a load takes whole sectors
+    constexpr bool HALVES = VEC && sizeof(SrcT) == 4;
     const int l = threadIdx.x & 15;
-    const SrcT *base = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + min(h, a.nkv - 1) * PR_HD + 8 * l;
+    const SrcT *base = static_cast<const SrcT *>(kv ? a.src_v : a.src_k) + min(h, a.nkv - 1) * PR_HD + (HALVES ? 4 : 8) * l;
     float x[STEPS][8];
     unsigned slot[STEPS];                // outside the pool: skipped
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int r = min(r0 + s * rows_step, a.n_rows - 1);
-        slot[s] = (unsigned)a.slot_map[r];
+        slot[s] = (unsigned)__ldcg(a.slot_map + r);
         const SrcT *src = base + (size_t)r * a.l_kvd;
         if constexpr (VEC && sizeof(SrcT) == 4) {
-            const float4 u = reinterpret_cast<const float4 *>(src)[0], v = reinterpret_cast<const float4 *>(src)[1];
+            const float4 u = __ldcg(reinterpret_cast<const float4 *>(src)), v = __ldcg(reinterpret_cast<const float4 *>(src + PR_HD / 2));
             x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
             x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
         } else if constexpr (VEC) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(src);
+            const uint4 u = __ldcg(reinterpret_cast<const uint4 *>(src));
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) { x[s][2 * k] = __uint_as_float(w[k] << 16); x[s][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[s][k] = load_as_f32(src + k);
+            for (int k = 0; k < 8; ++k) x[s][k] = load_cg(src + k);
         }
     }
     // Row maxima; lane l of a half keeps that of its step l % STEPS, so that the two divisions are done once for all steps.
@@ -102,7 +111,13 @@ __device__ __forceinline__ void append_rows(const PagedRowsArgs &a, int kv, int 
             }
         }
         const size_t row = ((size_t)(slot[s] / PR_PAGE) * a.nkv + h) * PR_PAGE + (size_t)(slot[s] % PR_PAGE);
-        reinterpret_cast<uint2 *>((kv ? a.v_pool : a.k_pool) + row * PR_HD)[l] = make_uint2(codes[0], codes[1]);
+        int8_t *dst = (kv ? a.v_pool : a.k_pool) + row * PR_HD;
+        if constexpr (HALVES) {
+            reinterpret_cast<uint32_t *>(dst)[l] = codes[0];
+            reinterpret_cast<uint32_t *>(dst + PR_HD / 2)[l] = codes[1];
+        } else {
+            reinterpret_cast<uint2 *>(dst)[l] = make_uint2(codes[0], codes[1]);
+        }
         if (l == 0) (kv ? a.vs_pool : a.ks_pool)[row] = sc;
     }
 }
@@ -182,9 +197,9 @@ __device__ __forceinline__ void page_bounds(const int8_t *k_pool, const float *k
 }
 
 // A decode step's rows (at most OWN_ROWS), and the bounds of the pages they complete, in one launch: a block takes every row of a
-// head, so all that a completed page holds of this call was written by the block itself.  64 rows x 16 heads: 3.2 us as two
-// launches (and 2 us more of host time).
-constexpr int OWN_ROWS = 256;
+// head, so all that a completed page holds of this call was written by the block itself.  64 rows x 16 heads: 3.0 us, 3.6 as two
+// launches (and 2 us more of host time); 200 rows 7.0 against 5.0.
+constexpr int OWN_ROWS = 128;
 template <typename SrcT, bool VEC>
 __global__ void __launch_bounds__(PR_WARPS * 32) append_head_i8_kernel(const __grid_constant__ PagedRowsArgs a, int8_t *kb_pool, float *kbs_pool) {
     __shared__ BoundsScratch sm;
@@ -204,53 +219,74 @@ __global__ void __launch_bounds__(PR_WARPS * 32) append_head_i8_kernel(const __g
     for (int k = 0; k < n; ++k) page_bounds(a.k_pool, a.ks_pool, kb_pool, kbs_pool, (size_t)s_pages[k] * a.nkv + h, sm);
 }
 
-struct PageBoundsArgs {
+// Longer appends: the K rows in a grid of their own (append_slots_i8_kernel), then this grid, whose blocks are V rows but for
+// `bound_blocks` of them behind the first `v_before`: each looks through 128 slots and works out the bounds of one head of the
+// pages that end there (one, in a prompt).  So the bounds, bound by latency, share the SMs with a stream of rows instead of
+// running after it, and V rows are written while the K grid drains: the K grid waited for its own predecessor before it let
+// this one be scheduled, so the slot map and the V rows' slots are settled.  Blocks are scheduled in order; those that wait for
+// the K grid come late enough not to hold up others.  Every bounds block waits: the grid ends after the K grid.
+// 8168 rows x 16 heads: bf16 26.9 us, fp32 30.6 (31.1 and 34.1 as all rows, then the bounds; bf16 27.6 with the bounds blocks first, 28.6 last).
+struct BoundsArgs {
+    int8_t *kb_pool;
+    float *kbs_pool;
+    int v_before, bound_blocks, row_blocks;      // row_blocks: blocks of one blockIdx.z of the row kernels
+};
+template <typename SrcT, bool VEC, int STEPS>
+__global__ void __launch_bounds__(PR_WARPS * 32) append_v_bounds_i8_kernel(const __grid_constant__ PagedRowsArgs a, const __grid_constant__ BoundsArgs bd) {
+    __shared__ BoundsScratch sm;
+    __shared__ int s_pages[PR_PAGE], s_n;
+    int block = blockIdx.x;
+    if (block < bd.v_before || block >= bd.v_before + bd.bound_blocks) {
+        asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+        if (block >= bd.v_before) block -= bd.bound_blocks;
+        const int z = block / bd.row_blocks, x = block - z * bd.row_blocks, hw = threadIdx.x >> 4;
+        const int rows_step = (2 * PR_WARPS) >> a.head_bits;
+        append_rows<SrcT, VEC, STEPS>(a, 1, 2 * PR_WARPS * z + (hw & ((1 << a.head_bits) - 1)), x * (rows_step * STEPS) + (hw >> a.head_bits), rows_step);
+        return;
+    }
+    block -= bd.v_before;
+    const int span = block / a.nkv, h = block - span * a.nkv;
+    if (threadIdx.x == 0) s_n = 0;
+    __syncthreads();
+    const int r = span * PR_PAGE + (int)threadIdx.x;
+    if ((int)threadIdx.x < PR_PAGE && r < a.n_rows) {
+        const unsigned slot = (unsigned)__ldcg(a.slot_map + r);
+        if (slot < a.n_slots && slot % PR_PAGE == PR_PAGE - 1) s_pages[atomicAdd(&s_n, 1)] = (int)(slot / PR_PAGE);   // any order: pages are independent
+    }
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    __syncthreads();
+    const int n = s_n;
+    for (int k = 0; k < n; ++k) page_bounds(a.k_pool, a.ks_pool, bd.kb_pool, bd.kbs_pool, (size_t)s_pages[k] * a.nkv + h, sm);
+}
+
+// Bounds of listed pages, a block per page and head.
+struct PageListArgs {
     const int8_t *k_pool;
     const float *ks_pool;
     int8_t *kb_pool;
     float *kbs_pool;
-    const int *list;                     // slots (a page is taken where its last row was written) or page ids
-    int n, nkv, span;                    // entries, and how many of them a block looks at
-    long n_pages;
-    int slots;
+    const int *pages;
+    int nkv, n_pages;
 };
-
-// grid (entry spans, KV heads): a block finds the pages of its span and works them out one after the other.
-__global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_constant__ PageBoundsArgs a) {
+__global__ void __launch_bounds__(PB_THREADS) page_bounds_kernel(const __grid_constant__ PageListArgs a) {
     __shared__ BoundsScratch sm;
-    __shared__ int s_pages[PB_THREADS], s_n;
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    // Slots: the preceding grid is the append of the same call, which waited for its own predecessor before it let this one be
-    // scheduled.  The slot map is settled then and looked through while the append still runs.  A page list may be the
-    // preceding grid's work.
-    if (!a.slots) asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const int i = blockIdx.x * a.span + threadIdx.x;
-    if ((int)threadIdx.x < a.span && i < a.n) {
-        const int v = __ldcg(a.list + i);
-        const bool last = !a.slots || (v >= 0 && v % PR_PAGE == PR_PAGE - 1);
-        const int page = a.slots ? v / PR_PAGE : v;
-        if (last && page >= 0 && page < a.n_pages) s_pages[atomicAdd(&s_n, 1)] = page;   // any order: pages are independent
-    }
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");              // (every block: the grid ends after the append)
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    __syncthreads();
-    const int n = s_n;
-    for (int k = 0; k < n; ++k)
-        page_bounds(a.k_pool, a.ks_pool, a.kb_pool, a.kbs_pool, (size_t)s_pages[k] * a.nkv + blockIdx.y, sm);
+    const int page = a.pages[blockIdx.x];
+    if (page < 0 || page >= a.n_pages) return;
+    page_bounds(a.k_pool, a.ks_pool, a.kb_pool, a.kbs_pool, (size_t)page * a.nkv + blockIdx.y, sm);
 }
 
-static int launch_bounds(cudaStream_t st, const PageBoundsArgs &in, const char *who) {
-    PageBoundsArgs a = in;
-    // In a decode step few rows end a page, in a prompt every 128th does: a block that looks at 128 slots finds about one.
-    a.span = a.slots ? PR_PAGE : 1;
+template <typename... P, typename... A>
+static int launch_rows(const char *who, cudaStream_t st, dim3 grid, void (*kernel)(P...), const A &...args) {
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((a.n + a.span - 1) / a.span, a.nkv); cfg.blockDim = dim3(PB_THREADS); cfg.stream = st;
+    cfg.gridDim = grid; cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
     cfg.attrs = pdl; cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, page_bounds_kernel, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) { set_error("%s: %s", who, cudaGetErrorString(e)); return NOMOS_ECUDA; }
     return NOMOS_OK;
@@ -258,48 +294,36 @@ static int launch_bounds(cudaStream_t st, const PageBoundsArgs &in, const char *
 
 int launch_page_bounds(cudaStream_t st, const void *k_pool, const void *ks_pool, void *kb_pool, void *kbs_pool, const int *pages, int n,
                        int nkv, int n_pages) {
-    return launch_bounds(st, PageBoundsArgs{static_cast<const int8_t *>(k_pool), static_cast<const float *>(ks_pool), static_cast<int8_t *>(kb_pool),
-                                            static_cast<float *>(kbs_pool), pages, n, nkv, 1, n_pages, 0}, "nomos_kv_paged_page_bounds_i8");
+    const PageListArgs a{static_cast<const int8_t *>(k_pool), static_cast<const float *>(ks_pool), static_cast<int8_t *>(kb_pool),
+                         static_cast<float *>(kbs_pool), pages, nkv, n_pages};
+    return launch_rows("nomos_kv_paged_page_bounds_i8", st, dim3(n, nkv), page_bounds_kernel, a);
+}
+
+template <typename SrcT, bool VEC>
+static int launch_append(cudaStream_t st, const PagedRowsArgs &a, int8_t *kb_pool, float *kbs_pool) {
+    const char *who = "nomos_kv_paged_append_rows_i8";
+    if (kb_pool != nullptr && a.n_rows <= OWN_ROWS) return launch_rows(who, st, dim3(a.nkv, 2), append_head_i8_kernel<SrcT, VEC>, a, kb_pool, kbs_pool);
+    // two sets of rows per block once one each would fill the GPU's warps several times over
+    const bool many = (long)a.n_rows * a.nkv > 2 * 148 * 64;
+    const int per_block = ((2 * PR_WARPS) >> a.head_bits) * (many ? 2 : 1);
+    const int row_blocks = (int)(((long)a.n_rows + per_block - 1) / per_block), z = (a.nkv + 2 * PR_WARPS - 1) / (2 * PR_WARPS);
+    int rc = launch_rows(who, st, dim3(row_blocks, kb_pool ? 1 : 2, z), many ? append_slots_i8_kernel<SrcT, VEC, 2> : append_slots_i8_kernel<SrcT, VEC, 1>, a);
+    if (rc != NOMOS_OK || kb_pool == nullptr) return rc;
+    BoundsArgs bd{kb_pool, kbs_pool, row_blocks * z / 2, (a.n_rows + PR_PAGE - 1) / PR_PAGE * a.nkv, row_blocks};
+    return launch_rows(who, st, dim3(row_blocks * z + bd.bound_blocks),
+                       many ? append_v_bounds_i8_kernel<SrcT, VEC, 2> : append_v_bounds_i8_kernel<SrcT, VEC, 1>, a, bd);
 }
 
 int launch_append_slots_i8(cudaStream_t st, const void *src_k, const void *src_v, void *k_pool, void *v_pool, void *ks_pool, void *vs_pool,
                            void *kb_pool, void *kbs_pool, const int *slot_map, int n_rows, int nkv, int l_kvd, int n_pages, int src_bf16) {
-    const char *who = "nomos_kv_paged_append_rows_i8";
     PagedRowsArgs a{src_k, src_v, static_cast<int8_t *>(k_pool), static_cast<int8_t *>(v_pool), static_cast<float *>(ks_pool),
                     static_cast<float *>(vs_pool), slot_map, n_rows, nkv, l_kvd, 0, (unsigned)n_pages * PR_PAGE};
     while (a.head_bits < 4 && (1 << a.head_bits) < nkv) ++a.head_bits;
     const bool vec = l_kvd % 8 == 0 && ((reinterpret_cast<uintptr_t>(src_k) | reinterpret_cast<uintptr_t>(src_v)) & 15) == 0;
-    // Two sets of rows per block once one each would fill the GPU's warps several times over.
-    const bool many = (long)n_rows * nkv > 2 * 148 * 64;
-    cudaLaunchAttribute pdl[1];
-    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    pdl[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    if (kb_pool != nullptr && n_rows <= OWN_ROWS) {
-        cfg.gridDim = dim3(nkv, 2); cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
-        cfg.attrs = pdl; cfg.numAttrs = 1;
-        void (*kernel)(PagedRowsArgs, int8_t *, float *) = src_bf16 ? (vec ? append_head_i8_kernel<__nv_bfloat16, true> : append_head_i8_kernel<__nv_bfloat16, false>)
-                                                                    : (vec ? append_head_i8_kernel<float, true> : append_head_i8_kernel<float, false>);
-        cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, static_cast<int8_t *>(kb_pool), static_cast<float *>(kbs_pool));
-        if (e == cudaSuccess) e = cudaGetLastError();
-        if (e != cudaSuccess) { set_error("%s: %s", who, cudaGetErrorString(e)); return NOMOS_ECUDA; }
-        return NOMOS_OK;
-    }
-    const int per_block = ((2 * PR_WARPS) >> a.head_bits) * (many ? 2 : 1);
-    cfg.gridDim = dim3((unsigned)(((long)n_rows + per_block - 1) / per_block), 2, (nkv + 2 * PR_WARPS - 1) / (2 * PR_WARPS));
-    cfg.blockDim = dim3(PR_WARPS * 32); cfg.stream = st;
-    cfg.attrs = pdl; cfg.numAttrs = 1;
-    void (*kernel)(PagedRowsArgs) =
-        src_bf16 ? (vec ? (many ? append_slots_i8_kernel<__nv_bfloat16, true, 2> : append_slots_i8_kernel<__nv_bfloat16, true, 1>)
-                        : (many ? append_slots_i8_kernel<__nv_bfloat16, false, 2> : append_slots_i8_kernel<__nv_bfloat16, false, 1>))
-                 : (vec ? (many ? append_slots_i8_kernel<float, true, 2> : append_slots_i8_kernel<float, true, 1>)
-                        : (many ? append_slots_i8_kernel<float, false, 2> : append_slots_i8_kernel<float, false, 1>));
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    if (e != cudaSuccess) { set_error("%s: %s", who, cudaGetErrorString(e)); return NOMOS_ECUDA; }
-    if (kb_pool == nullptr) return NOMOS_OK;
-    return launch_bounds(st, PageBoundsArgs{a.k_pool, a.ks_pool, static_cast<int8_t *>(kb_pool), static_cast<float *>(kbs_pool), slot_map, n_rows,
-                                            nkv, 0, n_pages, 1}, who);
+    int8_t *kb = static_cast<int8_t *>(kb_pool);
+    float *kbs = static_cast<float *>(kbs_pool);
+    if (src_bf16) return vec ? launch_append<__nv_bfloat16, true>(st, a, kb, kbs) : launch_append<__nv_bfloat16, false>(st, a, kb, kbs);
+    return vec ? launch_append<float, true>(st, a, kb, kbs) : launch_append<float, false>(st, a, kb, kbs);
 }
 
 }  // namespace nomos

@@ -162,7 +162,7 @@ def test_append_rows(dtype, nkv, gap, shift):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
-@pytest.mark.parametrize("nkv,rows,gap,shift", [(1, 1, 0, 0), (2, 256, 8, 0), (17, 130, 0, 0), (40, 64, 3, 1), (5, 257, 0, 0), (33, 700, 0, 2), (8, 3000, 16, 0)])
+@pytest.mark.parametrize("nkv,rows,gap,shift", [(1, 1, 0, 0), (2, 256, 8, 0), (17, 128, 0, 0), (16, 129, 0, 0), (40, 64, 3, 1), (5, 257, 0, 0), (33, 700, 0, 2), (8, 3000, 16, 0), (16, 2500, 0, 0)])
 def test_append_rows_up_to_page_ends(dtype, nkv, rows, gap, shift):
     """Few rows (one launch, a block per head) and many (two launches), head counts on both sides of a block's sixteen, pages completed over
     two calls, and untouched elsewhere."""
