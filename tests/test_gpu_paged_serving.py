@@ -197,6 +197,46 @@ def test_append_rows_up_to_page_ends(dtype, nkv, rows, gap, shift):
                 assert (host(pools[4])[p] == 99).all() and (host(pools[5])[p] == 77).all(), p
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("rows", [100, 1500])
+def test_append_rows_back_to_back(rows, captured):
+    """Sources rewritten right before every append and pools read right after it, nothing waited for: no call sees another one's rows."""
+    rng = np.random.default_rng(rows)
+    nkv, n_pages, rounds = 8, rows // PAGE + 3, 12
+    slots = i32(100 + np.arange(rows))
+    data = torch.from_numpy(rng.standard_normal((rounds, 2, rows, nkv, HD), dtype=np.float32)).to(DEV).to(torch.bfloat16)
+    src = torch.zeros_like(data[0])
+    pools = empty_pools(n_pages, nkv)
+    got = [[torch.empty_like(x) for x in pools] for _ in range(rounds)]
+
+    def step(i):
+        src.copy_(data[i])
+        ops.kv_paged_append_rows_i8(None, src[0], src[1], *pools, slots, n_rows=rows, nkv=nkv, l_hd=HD, l_kvd=nkv * HD, n_pages=n_pages, src_type=ops.BF16)
+        for x, y in zip(got[i], pools):
+            x.copy_(y)
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for i in range(rounds):
+                step(i)
+        for _ in range(2):
+            graph.replay()
+    else:
+        for i in range(rounds):
+            step(i)
+    torch.cuda.synchronize()
+    at = 100 + np.arange(rows)
+    for i in range(rounds):
+        for j in range(2):
+            code, scale = ref.codec(data[i, j].float().cpu().numpy())
+            assert np.array_equal(host(got[i][j])[at // PAGE, :, at % PAGE], code) and np.array_equal(host(got[i][2 + j])[at // PAGE, :, at % PAGE], scale), (i, j)
+        done = range(0, (100 + rows) // PAGE)
+        kb, kbs = ref.bounds(host(got[i][0]), host(got[i][2]))
+        for p in done:
+            assert np.array_equal(host(got[i][4])[p], kb[p]) and np.array_equal(host(got[i][5])[p], kbs[p]), (i, p)
+
+
 def test_append_rows_is_the_one_row_append():
     """The same codes and scales as the decode append, rows with infinities, NaN, zeros and denormals among them; no bounds asked for."""
     rng = np.random.default_rng(3)
