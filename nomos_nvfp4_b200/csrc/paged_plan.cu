@@ -218,7 +218,8 @@ int launch_paged_plan(cudaStream_t st, const int *seq_lens, const int *n_new, co
                  row_seq, row_pos, batch, max_pages, n_pages, max_rows, 0, 0};
     p.vec = ((reinterpret_cast<uintptr_t>(slot_map) | reinterpret_cast<uintptr_t>(row_seq) | reinterpret_cast<uintptr_t>(row_pos)) & 15) == 0;
     const size_t smem = (size_t)batch * 5 * sizeof(int);
-    cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_MAX_BATCH * 5 * (int)sizeof(int)) : cudaSuccess;
+    // (48 KB without the attribute, the kernel's own static arrays included)
+    cudaError_t e = smem > 40 * 1024 ? cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_MAX_BATCH * 5 * (int)sizeof(int)) : cudaSuccess;
     if (e != cudaSuccess) { set_error("nomos_kv_paged_plan: shared memory: %s", cudaGetErrorString(e)); return NOMOS_ECUDA; }
     const auto over = [](const void *x, long nx, const void *y, long ny) {
         const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);

@@ -73,9 +73,10 @@ def same_plan(d, want):
     assert int(host(d["free_count_out"])[0]) == want["free_count_out"]
 
 
+# (2440 before the larger ones: the first call whose shared memory needs the kernel's attribute is one of those just above 48 KB)
 @pytest.mark.parametrize("batch,max_pages,rows_each,finished,tight,extra", [
     (1, 1, 1, 0, False, 0), (1, 3, 200, 0, False, 9), (1, 3, 200, 1, False, 2), (7, 4, 1, 2, False, 0), (33, 9, 60, 5, True, 31),
-    (64, 32, 1, 0, False, 3), (100, 5, 130, 30, True, 1), (1000, 6, 9, 100, False, 0), (1025, 3, 40, 1, True, 7), (2500, 2, 3, 2500, False, 50),
+    (64, 32, 1, 0, False, 3), (100, 5, 130, 30, True, 1), (1000, 6, 9, 100, False, 0), (1025, 3, 40, 1, True, 7), (2050, 2, 1, 9, False, 0), (2440, 2, 1, 0, False, 5), (2457, 1, 2, 0, True, 0), (2500, 2, 3, 2500, False, 50),
     (5000, 4, 20, 77, True, 1), (8192, 2, 1, 0, False, 0), (40, 70, 1200, 3, False, 13), (40, 70, 1200, 3, True, -9000)])
 @pytest.mark.parametrize("alias,offset", [(False, 0), (True, 1)])
 def test_plan(batch, max_pages, rows_each, finished, tight, extra, alias, offset):
