@@ -400,6 +400,22 @@ def test_sparse_many_pages(pages, tops, alike):
         check_sparse(pools, q, row_seq, row_pos, got, sel, top=top, local=local)
 
 
+def test_sparse_most_pages():
+    """The longest context there is: 49152 pages, one physical page listed over and over between a few others."""
+    rng = np.random.default_rng(21)
+    pages, few = 49152, 12
+    pools = Pools(rng, [few * PAGE], 1)
+    phys = pools.table[0, :few].copy()
+    pools.lens, pools.max_pages = [pages * PAGE], pages
+    pools.table = np.full((1, pages), phys[0], np.int32)
+    pools.table[0, rng.choice(pages, 60, replace=False)] = rng.choice(phys[1:], 60)
+    row_seq, row_pos = np.array([0, 0]), np.array([pages * PAGE - 1, pages * PAGE - PAGE])
+    q = bf16_normal(rng, (2, 1, HD))
+    for top in (9, 300):
+        got, sel = run_sparse(pools, q, row_seq, row_pos, top=top)
+        check_sparse(pools, q, row_seq, row_pos, got, sel, top=top)
+
+
 def test_sparse_over_all_pages_is_paged_decode():
     """top_pages covering every sequence: dense attention, and the dense entry point's output (each within the bar of the exact one)."""
     rng = np.random.default_rng(8)
