@@ -491,7 +491,8 @@ int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks
  * that are not finite count as the largest finite value (a page of NaN keys is read, as dense attention would read it).
  * Every page but the row's last must have its bounds (see above).
  * sel_pages: 0, or [rows][nkv][top_pages], the page numbers within the sequence in ascending order, -1 beyond.
- * Accuracy of out: that of nomos_attn_paged_decode_i8 over the selected keys.  head_dim 128, at most 8 heads per KV head.
+ * Accuracy of out: that of nomos_attn_paged_decode_i8 over the selected keys.  head_dim 128, at most 8 heads per KV head, at most
+ * 2^30 rows.
  * The workspace (16-byte aligned) must not be shared by calls that can overlap on the GPU. */
 int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t top_pages,
                                                 int32_t max_len);
@@ -514,7 +515,7 @@ int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_sparse_t *args
  * W_i = rint(weight_i * 2^50), T = floor(u_sample * sum W) in 64 bits, the first token with W_0 + .. + W_i > T; -1 if all are
  * zero.  Whole-number sums make it independent of how the row is split.
  * seq_lens_out[b] = seq_lens[b] + a + 1, the keys that stay cached once the last sampled token's row and the accepted drafts'
- * rows are (seq_lens may be seq_lens_out; both 0: no lengths). */
+ * rows are (seq_lens may be seq_lens_out; both 0: no lengths).  max_draft and vocab are at most 2^30. */
 typedef struct nomos_attn_verify {
     uint64_t struct_bytes;
     uint64_t target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens;

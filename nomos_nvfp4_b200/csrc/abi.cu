@@ -783,6 +783,7 @@ NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_s
                 c->row_pos && c->out && c->workspace, "%s: null pointer", who);
     REQUIRE(fits32({c->rows, c->batch, c->nh, c->nkv, c->kvg, c->l_hd, c->n_pages, c->max_pages, c->max_len, c->top_pages, c->sink_pages,
                     c->local_pages}), "%s: dimensions are 32-bit numbers", who);
+    REQUIRE(c->rows <= (1l << 30), "%s: %ld rows in one call", who, (long)c->rows);
     int rc = check_page_pool(who, c->nkv, c->l_hd, c->n_pages);
     if (rc) return rc;
     REQUIRE((c->q_type == ET_F32 || c->q_type == ET_BF16) && (c->out_type == ET_F32 || c->out_type == ET_BF16), "%s: element type", who);
@@ -841,7 +842,9 @@ NOMOS_EXPORT int32_t nomos_attn_spec_verify(void *stream, const nomos_attn_verif
     const char *who = "nomos_attn_spec_verify";
     REQUIRE_BLOCK(a, nomos_attn_verify_t);
     if (a->batch <= 0) return NOMOS_OK;
-    REQUIRE(fits32({a->batch, a->max_draft, a->vocab}) && a->max_draft >= 0 && a->max_draft < 0x7fffffff && a->vocab > 0, "%s: bad max_draft/vocab", who);
+    // (the kernel's 32-bit indices step up to a batch of loads past the last element)
+    REQUIRE(fits32({a->batch, a->max_draft, a->vocab}) && a->max_draft >= 0 && a->max_draft <= (1l << 30) && a->vocab > 0 && a->vocab <= (1l << 30),
+            "%s: bad max_draft/vocab", who);
     REQUIRE(a->target_probs && a->u_sample && a->n_accepted && a->out_tokens && (a->max_draft == 0 || (a->draft_tokens && a->u_accept)),
             "%s: null pointer", who);
     REQUIRE((a->seq_lens != 0) == (a->seq_lens_out != 0), "%s: lengths need an input and an output", who);
