@@ -512,8 +512,9 @@ int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_sparse_t *args
  * Draft i of token x is accepted iff u_accept * q_i(x) < p_i(x), in 64 bits; a token outside [0, vocab) is rejected.  With a
  * the first one rejected (n_draft if none): n_accepted[b] = a, out_tokens [batch][max_draft + 1] = the a accepted tokens, then
  * one drawn from max(p_a - q_a, 0) -- from p_a where none was rejected, or where that is zero throughout -- then -1.  The draw:
- * W_i = rint(weight_i * 2^50), T = floor(u_sample * sum W) in 64 bits, the first token with W_0 + .. + W_i > T; -1 if all are
- * zero.  Whole-number sums make it independent of how the row is split.
+ * W_i = rint(weight_i * 2^50) (a probability p above 1, as rounding may leave it, counts as 1), T = floor(u_sample * sum W) in
+ * 64 bits, the first token with W_0 + .. + W_i > T; -1 if all are zero.  Whole-number sums make it independent of how the row is
+ * split.
  * seq_lens_out[b] = seq_lens[b] + a + 1, the keys that stay cached once the last sampled token's row and the accepted drafts'
  * rows are (seq_lens may be seq_lens_out; both 0: no lengths).  max_draft and vocab are at most 2^30. */
 typedef struct nomos_attn_verify {

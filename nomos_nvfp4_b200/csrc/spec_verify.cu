@@ -33,10 +33,13 @@ struct SpecVerifyArgs {
 
 // Adds the whole weight of max(p - q, 0) to a sum.  6 + (p - q) lies in [4, 8), whose doubles are 2^-50 apart: the addition
 // rounds to whole units, and the bit pattern less that of 6.0 (whose low word is zero) is their number.  (A conversion to a
-// 64-bit integer is slower.)  p above 1 counts as 1, NaN as nothing.
+// 64-bit integer is slower.)  p above 1 counts as 1, and only then is compared: q may be above 1 as well, and a negative difference
+// would wrap.  A NaN stays one through the minimum and compares false: it weighs nothing.
 __device__ __forceinline__ void add_weight(unsigned long long &sum, float p, float q) {
-    const long long u = __double_as_longlong(__dadd_rn(__dsub_rn((double)fminf(p, 1.0f), (double)q), 6.0));
-    if (p > q) sum += (unsigned long long)(u - 0x4018000000000000ll);
+    float pc;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(pc) : "f"(p), "f"(1.0f));
+    const long long u = __double_as_longlong(__dadd_rn(__dsub_rn((double)pc, (double)q), 6.0));
+    if (pc > q) sum += (unsigned long long)(u - 0x4018000000000000ll);
 }
 
 // One row's weights: target row, drafter row (nullptr: none), and the index whose drafter probability is 1 (a drafter that
@@ -177,7 +180,8 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
         const unsigned long long total = __shfl_sync(0xffffffffu, upto, 31);
         const unsigned long long after = __shfl_sync(0xffffffffu, upto, rank), before = after - s_total[round];
         if (total == 0 && round == 0 && (w.q || w.one >= 0)) {
-            // the drafter covers the target everywhere (u outside [0, 1) only): the target's own row decides
+            // nothing is left of the target's row: the drafter covers it everywhere (equal rows and a drafted token of probability 0
+            // in both, or one that is none), by less than 2^-51 at most, or u was outside [0, 1).  The target's own row decides
             w.q = nullptr; w.one = -1;
             continue;
         }
