@@ -516,11 +516,20 @@ int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_sparse_t *args
  * 64 bits, the first token with W_0 + .. + W_i > T; -1 if all are zero.  Whole-number sums make it independent of how the row is
  * split.
  * seq_lens_out[b] = seq_lens[b] + a + 1, the keys that stay cached once the last sampled token's row and the accepted drafts'
- * rows are (seq_lens may be seq_lens_out; both 0: no lengths).  max_draft and vocab are at most 2^30. */
+ * rows are (seq_lens may be seq_lens_out; both 0: no lengths).  max_draft and vocab are at most 2^30.
+ * granted: 0, or what nomos_kv_paged_plan wrote, rows placed [batch], so that nothing has to be read back between the two.  A
+ * sequence's rows are then its new tokens (the last one sampled, or a prompt chunk) followed by its n drafts:
+ *   granted[b] <= 0: nothing was computed for it (no pages, finished, idle); nothing of it is written.
+ *   n_draft[b] < 0: its rows stay, no token is drawn (a prompt chunk that is not the last): seq_lens_out[b] = seq_lens[b] +
+ *     granted[b], nothing else is written.
+ *   otherwise n is at most granted[b] - 1, and seq_lens_out[b] = seq_lens[b] + granted[b] - n + a.  (Row i of target_probs belongs
+ *     to the sequence's row granted[b] - 1 - n + i; a prompt's last chunk has n_draft 0.)
+ * struct_bytes may be that of a block without the field, which means 0. */
 typedef struct nomos_attn_verify {
     uint64_t struct_bytes;
     uint64_t target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens;
     int64_t batch, max_draft, vocab, p_stride, q_stride;
+    uint64_t granted;
 } nomos_attn_verify_t;
 int32_t nomos_attn_spec_verify(void *stream, const nomos_attn_verify_t *args);
 

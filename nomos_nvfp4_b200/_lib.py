@@ -81,7 +81,7 @@ class AttnVerify(C.Structure):
     """Mirror of ``nomos_attn_verify_t``."""
     _fields_ = [("struct_bytes", u64), ("target_probs", u64), ("draft_probs", u64), ("draft_tokens", u64), ("n_draft", u64), ("u_accept", u64),
                 ("u_sample", u64), ("seq_lens", u64), ("seq_lens_out", u64), ("n_accepted", u64), ("out_tokens", u64), ("batch", i64),
-                ("max_draft", i64), ("vocab", i64), ("p_stride", i64), ("q_stride", i64)]
+                ("max_draft", i64), ("vocab", i64), ("p_stride", i64), ("q_stride", i64), ("granted", u64)]
 
 
 def packer(block) -> struct.Struct:

@@ -2,6 +2,7 @@
 // Declarations and per-function reference citations live in include/nomos_attn.h.
 #include <algorithm>
 #include <cstdarg>
+#include <cstddef>
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -840,7 +841,11 @@ NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_s
 
 NOMOS_EXPORT int32_t nomos_attn_spec_verify(void *stream, const nomos_attn_verify_t *a) {
     const char *who = "nomos_attn_spec_verify";
-    REQUIRE_BLOCK(a, nomos_attn_verify_t);
+    // a block that ends before `granted` (callers built without it) has none
+    constexpr uint64_t without_granted = offsetof(nomos_attn_verify_t, granted);
+    REQUIRE(a != nullptr && (a->struct_bytes == sizeof(nomos_attn_verify_t) || a->struct_bytes == without_granted), "%s: argument block of another version",
+            who);
+    const uint64_t granted = a->struct_bytes == without_granted ? 0 : a->granted;
     if (a->batch <= 0) return NOMOS_OK;
     // (the kernel's 32-bit indices step up to a batch of loads past the last element)
     REQUIRE(fits32({a->batch, a->max_draft, a->vocab}) && a->max_draft >= 0 && a->max_draft <= (1l << 30) && a->vocab > 0 && a->vocab <= (1l << 30),
@@ -850,12 +855,12 @@ NOMOS_EXPORT int32_t nomos_attn_spec_verify(void *stream, const nomos_attn_verif
     REQUIRE((a->seq_lens != 0) == (a->seq_lens_out != 0), "%s: lengths need an input and an output", who);
     REQUIRE(a->p_stride >= a->vocab && (!a->draft_probs || a->q_stride >= a->vocab), "%s: rows of %ld probabilities, fewer apart", who, (long)a->vocab);
     for (uint64_t x : {a->target_probs, a->draft_probs, a->draft_tokens, a->n_draft, a->u_accept, a->u_sample, a->seq_lens, a->seq_lens_out,
-                       a->n_accepted, a->out_tokens})
+                       a->n_accepted, a->out_tokens, granted})
         REQUIRE(aligned(x, 4), "%s: misaligned buffer", who);
     const auto f = [](uint64_t x) { return static_cast<const float *>(ptr(x)); };
     const auto i = [](uint64_t x) { return static_cast<int *>(ptr(x)); };
     return launch_spec_verify(as_stream(stream), f(a->target_probs), a->max_draft > 0 ? f(a->draft_probs) : nullptr, i(a->draft_tokens),
-                              i(a->n_draft), f(a->u_accept), f(a->u_sample), i(a->seq_lens), i(a->seq_lens_out), i(a->n_accepted),
+                              i(a->n_draft), f(a->u_accept), f(a->u_sample), i(a->seq_lens), i(granted), i(a->seq_lens_out), i(a->n_accepted),
                               i(a->out_tokens), (int)a->batch, (int)a->max_draft, (int)a->vocab, a->p_stride, a->q_stride);
 }
 

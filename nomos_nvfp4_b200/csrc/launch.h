@@ -44,8 +44,8 @@ struct PagedSelect {
 int launch_paged_select(cudaStream_t st, const PagedSelect &s);
 // ---- spec_verify.cu
 int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const int *tokens, const int *n_draft, const float *u_accept,
-                       const float *u_sample, const int *lens, int *lens_out, int *n_accepted, int *out_tokens, int batch, int max_draft,
-                       int vocab, long p_stride, long q_stride);
+                       const float *u_sample, const int *lens, const int *granted, int *lens_out, int *n_accepted, int *out_tokens, int batch,
+                       int max_draft, int vocab, long p_stride, long q_stride);
 int launch_append_i4(cudaStream_t st, const void *src_k, const void *src_v, void *dst_k, void *dst_v, void *k_scales,
                      void *v_scales, void *k_q8, void *v_q8, void *k_q8_scales, void *v_q8_scales, int n_s, int nkv,
                      int l_hd, int l_kvd, int cache_cap, int cache_hd, int base_pos, int q8_pitch, int scale_blocks);

@@ -25,7 +25,7 @@ struct SpecVerifyArgs {
     const float *p, *q;                  // [batch][max_draft + 1][p_stride], [batch][max_draft][q_stride] or nullptr
     const int *tokens, *n_draft;
     const float *u_accept, *u_sample;
-    const int *lens;
+    const int *lens, *granted;           // granted: rows the step placed for the sequence, or nullptr
     int *lens_out, *n_accepted, *out_tokens;
     int batch, max_draft, vocab;
     long p_stride, q_stride;
@@ -121,8 +121,14 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int b = blockIdx.y, rank = blockIdx.x, C = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n = min(a.n_draft ? a.n_draft[b] : a.max_draft, a.max_draft);
+    int n = min(a.n_draft ? a.n_draft[b] : a.max_draft, a.max_draft), rows = n + 1;
     const float u_sample = a.u_sample[b];
+    if (a.granted) {                     // a request that got no pages has no rows: its probabilities are not to be read
+        rows = a.granted[b];
+        if (rows <= 0) return;
+        n = min(n, rows - 1);            // (a draft whose row was not placed has not been looked at)
+        if (n < 0 && a.lens && rank == 0 && threadIdx.x == 0) a.lens_out[b] = a.lens[b] + rows;   // part of a prompt: cached, no token
+    }
     if (n < 0) return;                   // an idle entry of a padded batch; the whole cluster leaves
     // ---- how many drafts stand: every CTA of the cluster finds out for itself
     if (warp == 0) {
@@ -225,15 +231,15 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
             if (i != acc) a.out_tokens[(size_t)b * (a.max_draft + 1) + i] = i < acc ? a.tokens[(size_t)b * a.max_draft + i] : -1;
         if (threadIdx.x == 0) {
             a.n_accepted[b] = acc;
-            if (a.lens) a.lens_out[b] = a.lens[b] + acc + 1;
+            if (a.lens) a.lens_out[b] = a.lens[b] + rows - n + acc;
         }
     }
     cluster.sync();                      // the totals stay where the peers read them
 }
 
 int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const int *tokens, const int *n_draft, const float *u_accept,
-                       const float *u_sample, const int *lens, int *lens_out, int *n_accepted, int *out_tokens, int batch, int max_draft,
-                       int vocab, long p_stride, long q_stride) {
+                       const float *u_sample, const int *lens, const int *granted, int *lens_out, int *n_accepted, int *out_tokens, int batch,
+                       int max_draft, int vocab, long p_stride, long q_stride) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -260,8 +266,8 @@ int launch_spec_verify(cudaStream_t st, const float *p, const float *q, const in
         const int nb = std::min(65535, batch - b0);
         SpecVerifyArgs a{p + (size_t)b0 * (max_draft + 1) * p_stride, q ? q + (size_t)b0 * max_draft * q_stride : nullptr,
                          tokens + (size_t)b0 * max_draft, n_draft ? n_draft + b0 : nullptr, u_accept + (size_t)b0 * max_draft, u_sample + b0,
-                         lens ? lens + b0 : nullptr, lens_out ? lens_out + b0 : nullptr, n_accepted + b0, out_tokens + (size_t)b0 * (max_draft + 1),
-                         nb, max_draft, vocab, p_stride, q_stride};
+                         lens ? lens + b0 : nullptr, granted ? granted + b0 : nullptr, lens_out ? lens_out + b0 : nullptr, n_accepted + b0,
+                         out_tokens + (size_t)b0 * (max_draft + 1), nb, max_draft, vocab, p_stride, q_stride};
         attr[1].val.clusterDim.x = ctas;
         cfg.gridDim = dim3(ctas, nb);
         cudaError_t e = cudaLaunchKernelEx(&cfg, spec_verify_kernel, a);

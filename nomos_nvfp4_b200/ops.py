@@ -394,12 +394,14 @@ def attn_paged_sparse_i8(stream, q, k_pool, v_pool, ks_pool, vs_pool, kb_pool, k
 
 
 def spec_verify(stream, target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens, *,
-                batch, max_draft, vocab, p_stride, q_stride):
+                batch, max_draft, vocab, p_stride, q_stride, granted=None):
     """Speculative verification from given random numbers: accepted drafts, and the next token from the residual (or, all
-    accepted, from the target's last row); see include/nomos_attn.h.  ``draft_probs``, ``n_draft``, ``seq_lens`` may be ``None``."""
+    accepted, from the target's last row); see include/nomos_attn.h.  ``draft_probs``, ``n_draft``, ``seq_lens`` may be ``None``.
+    With the plan's ``granted`` a request that got no pages is left alone and lengths grow by the rows that were placed, less the
+    drafts that fall (``n_draft`` < 0: a prompt chunk that asks for no token)."""
     _check(_lib.lib().nomos_attn_spec_verify(_stream(stream), _VERIFY.pack(
         _VERIFY.size, *_addrs(target_probs, draft_probs, draft_tokens, n_draft, u_accept, u_sample, seq_lens, seq_lens_out, n_accepted, out_tokens),
-        batch, max_draft, vocab, p_stride, q_stride)))
+        batch, max_draft, vocab, p_stride, q_stride, _addr(granted))))
 
 
 class KvRing:
