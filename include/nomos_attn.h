@@ -493,7 +493,8 @@ int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks
  * sel_pages: 0, or [rows][nkv][top_pages], the page numbers within the sequence in ascending order, -1 beyond.
  * Accuracy of out: that of nomos_attn_paged_decode_i8 over the selected keys.  head_dim 128, at most 8 heads per KV head, at most
  * 2^30 rows.
- * The workspace (16-byte aligned) must not be shared by calls that can overlap on the GPU. */
+ * The workspace (16-byte aligned) must not be shared by calls that can overlap on the GPU.  The bytes asked for `rows` also serve
+ * every call of fewer rows, the other arguments alike. */
 int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t top_pages,
                                                 int32_t max_len);
 typedef struct nomos_attn_sparse {

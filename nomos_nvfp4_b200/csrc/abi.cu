@@ -764,9 +764,10 @@ NOMOS_EXPORT int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32
                                                              int32_t top_pages, int32_t max_len) {
     const char *who = "nomos_attn_paged_sparse_workspace_bytes";
     if (rows <= 0) return 0;
+    // What every row count up to this one needs, so that a buffer sized for the largest step serves the smaller ones (and the last
+    // launch of a long call): fewer rows are split more, and may need more.  Host arithmetic, at most some milliseconds.
     int64_t most = 0;
-    for (int r : {std::min(rows, SPARSE_ROWS), rows % SPARSE_ROWS}) {   // full launches, and the last one with its own split
-        if (r == 0) continue;
+    for (int r = 1; r <= std::min(rows, SPARSE_ROWS); ++r) {
         AttnArgs a;
         SparseWs w;
         int rc = fill_sparse(a, w, who, r, nh, nkv, kvg, l_hd, 1, top_pages, max_len);

@@ -376,6 +376,7 @@ def kv_paged_page_bounds_i8(stream, k_pool, ks_pool, kb_pool, kbs_pool, pages, *
 
 
 def attn_paged_sparse_workspace_bytes(*, rows, nh, nkv, kvg, l_hd, top_pages, max_len) -> int:
+    """Bytes for calls of up to ``rows`` rows: ask once, for the largest step."""
     n = _lib.lib().nomos_attn_paged_sparse_workspace_bytes(rows, nh, nkv, kvg, l_hd, top_pages, max_len)
     if n < 0:
         _check(int(n))
