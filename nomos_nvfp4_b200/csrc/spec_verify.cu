@@ -118,18 +118,24 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ unsigned long long s_warp[2][SV_WARPS], s_total[2], s_scan[SV_WARPS];
     __shared__ int s_accepted;
+    __shared__ float s_u;                // (every register counts here: forty per thread, so that three CTAs share an SM)
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int b = blockIdx.y, rank = blockIdx.x, C = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int n = min(a.n_draft ? a.n_draft[b] : a.max_draft, a.max_draft), rows = n + 1;
-    const float u_sample = a.u_sample[b];
-    if (a.granted) {                     // a request that got no pages has no rows: its probabilities are not to be read
-        rows = a.granted[b];
-        if (rows <= 0) return;
-        n = min(n, rows - 1);            // (a draft whose row was not placed has not been looked at)
-        if (n < 0 && a.lens && rank == 0 && threadIdx.x == 0) a.lens_out[b] = a.lens[b] + rows;   // part of a prompt: cached, no token
+    // Drafts to look at (a draft whose row was not placed is none), and the rows that stay whatever becomes of them.
+    const auto counts = [&](int &other) {
+        const int k = min(a.n_draft ? a.n_draft[b] : a.max_draft, a.max_draft), rows = a.granted ? a.granted[b] : k + 1;
+        const int m = rows > 0 ? min(k, rows - 1) : -1;
+        other = rows - max(m, 0);
+        return m;
+    };
+    int other;
+    const int n = counts(other);
+    if (threadIdx.x == SV_THREADS - 1) s_u = a.u_sample[b];
+    if (n < 0) {                         // idle, or without pages: nothing of it is read or written; the whole cluster leaves
+        if (a.granted && other > 0 && a.lens && rank == 0 && threadIdx.x == 0) a.lens_out[b] = a.lens[b] + other;   // part of a prompt
+        return;
     }
-    if (n < 0) return;                   // an idle entry of a padded batch; the whole cluster leaves
     // ---- how many drafts stand: every CTA of the cluster finds out for itself
     if (warp == 0) {
         int acc = n;
@@ -160,10 +166,10 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
     // stretch of this warp: [i0, i1) of the vocabulary, cut where the target row crosses 16-byte boundaries (`lead` elements
     // precede the first one; they belong to the first warp)
     const int lead = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(w.p) & 15)) & 15) / 4);
-    const int per = (int)((((long)a.vocab + (long)C * SV_WARPS - 1) / ((long)C * SV_WARPS) + 3) / 4 * 4);
-    const auto cut = [&](long unit) { return unit == 0 ? 0 : (int)min(unit * per + lead, (long)a.vocab); };
-    const long unit = (long)rank * SV_WARPS + warp;
-    const int i0 = cut(unit), i1 = unit == (long)C * SV_WARPS - 1 ? a.vocab : cut(unit + 1);
+    const int per = ((a.vocab + C * SV_WARPS - 1) / (C * SV_WARPS) + 3) / 4 * 4;                 // (vocab <= 2^30: 32 bits hold it all)
+    const auto cut = [&](int unit) { return unit == 0 ? 0 : min(unit * per + lead, a.vocab); };
+    const int unit = rank * SV_WARPS + warp;
+    const int i0 = cut(unit), i1 = unit == C * SV_WARPS - 1 ? a.vocab : cut(unit + 1);
 
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
             continue;
         }
         if (total > 0) {
-            const long long t0 = (long long)floor(__dmul_rn((double)u_sample, (double)total));
+            const long long t0 = (long long)floor(__dmul_rn((double)s_u, (double)total));
             const unsigned long long T = (unsigned long long)max(0ll, min(t0, (long long)total - 1));
             if (T >= before && T < after) {                           // uniform over the CTA
                 // the warp whose stretch holds T
@@ -200,8 +206,8 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
                 const int k = min(SV_WARPS - 1, __popc(__ballot_sync(0xffffffffu, lane < SV_WARPS && T >= w_upto)));
                 unsigned long long base = __shfl_sync(0xffffffffu, w_upto - mine_w, k);
                 // the k-th warp's stretch again, by the whole CTA: `each` neighbouring elements per thread
-                const long u0 = (long)rank * SV_WARPS + k;
-                const int j0 = cut(u0), j1 = u0 == (long)C * SV_WARPS - 1 ? a.vocab : cut(u0 + 1);
+                const int u0 = rank * SV_WARPS + k;
+                const int j0 = cut(u0), j1 = u0 == C * SV_WARPS - 1 ? a.vocab : cut(u0 + 1);
                 const int each = (j1 - j0 + SV_THREADS - 1) / SV_THREADS;
                 const int e0 = min(j1, j0 + (int)threadIdx.x * each), e1 = min(j1, e0 + each);
                 unsigned long long s = 0;
@@ -231,7 +237,10 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
             if (i != acc) a.out_tokens[(size_t)b * (a.max_draft + 1) + i] = i < acc ? a.tokens[(size_t)b * a.max_draft + i] : -1;
         if (threadIdx.x == 0) {
             a.n_accepted[b] = acc;
-            if (a.lens) a.lens_out[b] = a.lens[b] + rows - n + acc;
+            if (a.lens) {                // (asked for again rather than kept in a register over the streams)
+                counts(other);
+                a.lens_out[b] = a.lens[b] + other + acc;
+            }
         }
     }
     cluster.sync();                      // the totals stay where the peers read them
