@@ -5,7 +5,7 @@
 // q . k of every key of the page.  A page with a row scale that is not finite gets t = +inf and codes 0.
 // Both are streams: a row is read once and written once, a completed page's K codes are read back once, mostly out of L2.
 // 8168 rows x 16 heads: fp32 rows 26 us (6.4 TB/s, close to the copy rate), bf16 rows 22 us (4.6 TB/s, bound by instruction issue); the bounds
-// of their 1024 pages and heads 10 us alone (17 MB; latency and the ALU pipe), 5 beside the V rows.
+// of their 1024 pages and heads 10 us alone (17 MB; latency and the ALU pipe), 6 beside the V rows.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -52,8 +52,7 @@ __device__ __forceinline__ float load_cg(const __nv_bfloat16 *p) {
 // Half a warp per row of one (K or V, KV head): lane l holds elements 8l .. 8l + 7, one or two wide loads and one 8-byte store of
 // codes.  The half warp takes rows r0, r0 + rows_step, ... (STEPS of them, loaded before the first use).
 // VEC: rows start on a boundary of eight elements; otherwise the same elements one by one.
-// Everything is read through L2 (ld.global.cg): nothing is read twice, and the V rows of a long append are read in a grid that
-// does not itself wait for their producer (append_v_bounds_i8_kernel).
+// Everything is read through L2 (ld.global.cg): nothing is read twice.
 template <typename SrcT, bool VEC, int STEPS>
 __device__ __forceinline__ void append_rows(const PagedRowsArgs &a, int kv, int h, int r0, int rows_step) {
     // wide fp32 loads: lane l holds elements 4l .. 4l + 3 of each half of the row, so that a load takes whole sectors
@@ -219,42 +218,39 @@ __global__ void __launch_bounds__(PR_WARPS * 32) append_head_i8_kernel(const __g
     for (int k = 0; k < n; ++k) page_bounds(a.k_pool, a.ks_pool, kb_pool, kbs_pool, (size_t)s_pages[k] * a.nkv + h, sm);
 }
 
-// Longer appends: the K rows in a grid of their own (append_slots_i8_kernel), then this grid, whose blocks are V rows but for
-// `bound_blocks` of them behind the first `v_before`: each looks through 128 slots and works out the bounds of one head of the
-// pages that end there (one, in a prompt).  So the bounds, bound by latency, share the SMs with a stream of rows instead of
-// running after it, and V rows are written while the K grid drains: the K grid waited for its own predecessor before it let
-// this one be scheduled, so the slot map and the V rows' slots are settled.  Blocks are scheduled in order; those that wait for
-// the K grid come late enough not to hold up others.  Every bounds block waits: the grid ends after the K grid.
-// 8168 rows x 16 heads: bf16 26.9 us, fp32 30.6 (31.1 and 34.1 as all rows, then the bounds; bf16 27.6 with the bounds blocks first, 28.6 last).
+// Longer appends: the K rows in a grid of their own (append_slots_i8_kernel), then this grid, whose first `bound_blocks` blocks each
+// look through 128 slots and work out the bounds of one head of the pages that end there (one, in a prompt); the others are V rows.
+// So the bounds, bound by latency, share the SMs with a stream of rows instead of running after it.  Every block waits for the K grid:
+// the bounds blocks read its rows, and for the V rows nothing else promises that what the calls before wrote (sources, slots) is
+// visible.  8168 rows x 16 heads: bf16 28.3 us, fp32 33.0 (bounds blocks in the middle of the V rows 0.9 and 0.6 more; all rows in one
+// grid, then the bounds, 31.1 and 34.1; V rows and slots read without the wait, 26.8 and 30.6).
 struct BoundsArgs {
     int8_t *kb_pool;
     float *kbs_pool;
-    int v_before, bound_blocks, row_blocks;      // row_blocks: blocks of one blockIdx.z of the row kernels
+    int bound_blocks, row_blocks;        // row_blocks: blocks of one blockIdx.z of the row kernels
 };
 template <typename SrcT, bool VEC, int STEPS>
 __global__ void __launch_bounds__(PR_WARPS * 32) append_v_bounds_i8_kernel(const __grid_constant__ PagedRowsArgs a, const __grid_constant__ BoundsArgs bd) {
     __shared__ BoundsScratch sm;
     __shared__ int s_pages[PR_PAGE], s_n;
     int block = blockIdx.x;
-    if (block < bd.v_before || block >= bd.v_before + bd.bound_blocks) {
-        asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-        if (block >= bd.v_before) block -= bd.bound_blocks;
+    if (threadIdx.x == 0) s_n = 0;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    if (block >= bd.bound_blocks) {
+        block -= bd.bound_blocks;
         const int z = block / bd.row_blocks, x = block - z * bd.row_blocks, hw = threadIdx.x >> 4;
         const int rows_step = (2 * PR_WARPS) >> a.head_bits;
         append_rows<SrcT, VEC, STEPS>(a, 1, 2 * PR_WARPS * z + (hw & ((1 << a.head_bits) - 1)), x * (rows_step * STEPS) + (hw >> a.head_bits), rows_step);
         return;
     }
-    block -= bd.v_before;
     const int span = block / a.nkv, h = block - span * a.nkv;
-    if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
     const int r = span * PR_PAGE + (int)threadIdx.x;
     if ((int)threadIdx.x < PR_PAGE && r < a.n_rows) {
         const unsigned slot = (unsigned)__ldcg(a.slot_map + r);
         if (slot < a.n_slots && slot % PR_PAGE == PR_PAGE - 1) s_pages[atomicAdd(&s_n, 1)] = (int)(slot / PR_PAGE);   // any order: pages are independent
     }
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     __syncthreads();
     const int n = s_n;
     for (int k = 0; k < n; ++k) page_bounds(a.k_pool, a.ks_pool, bd.kb_pool, bd.kbs_pool, (size_t)s_pages[k] * a.nkv + h, sm);
@@ -309,7 +305,7 @@ static int launch_append(cudaStream_t st, const PagedRowsArgs &a, int8_t *kb_poo
     const int row_blocks = (int)(((long)a.n_rows + per_block - 1) / per_block), z = (a.nkv + 2 * PR_WARPS - 1) / (2 * PR_WARPS);
     int rc = launch_rows(who, st, dim3(row_blocks, kb_pool ? 1 : 2, z), many ? append_slots_i8_kernel<SrcT, VEC, 2> : append_slots_i8_kernel<SrcT, VEC, 1>, a);
     if (rc != NOMOS_OK || kb_pool == nullptr) return rc;
-    BoundsArgs bd{kb_pool, kbs_pool, row_blocks * z / 2, (a.n_rows + PR_PAGE - 1) / PR_PAGE * a.nkv, row_blocks};
+    const BoundsArgs bd{kb_pool, kbs_pool, (a.n_rows + PR_PAGE - 1) / PR_PAGE * a.nkv, row_blocks};
     return launch_rows(who, st, dim3(row_blocks * z + bd.bound_blocks),
                        many ? append_v_bounds_i8_kernel<SrcT, VEC, 2> : append_v_bounds_i8_kernel<SrcT, VEC, 1>, a, bd);
 }
