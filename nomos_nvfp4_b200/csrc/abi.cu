@@ -828,7 +828,7 @@ NOMOS_EXPORT int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_s
         a.out = ptr(c->out + (uint64_t)r0 * nh * l_hd * os);
         a.block_table = s.lists; a.seq_lens = s.lens;
         // as many rows for each sequence as there is room for, the rest padding: exact for decode and verify steps padded to a
-        // captured size, and nothing but the split depends on it
+        // captured size, a guess where sequences bring different numbers of rows.  Nothing but the split depends on it
         a.live_rows = nr > c->batch ? nr / (int)c->batch * (int)c->batch : 0;
         a.workspace = ptr(c->workspace + w.lists + w.lens); a.ws_bytes = w.attn;
         a.softmax_scale = (float)c->softmax_scale; a.q_type = (int)c->q_type; a.out_type = (int)c->out_type;

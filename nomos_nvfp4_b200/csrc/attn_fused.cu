@@ -683,7 +683,9 @@ static int launch_tc5_inst(cudaStream_t st, const AttnArgs &a, bool query_ws, lo
     // evict-first tile copies protect what the launch comes back to (code, query, partials) from its own stream:
     // verify at 16393 keys 26.5 -> 25.7 us; on streams of gigabytes, where that fixed part is noise, they measured
     // 3 % slower (C5a 612 -> 630 us, C5b 312 -> 323 us), hence the size limit (554 MB: 87.6 -> 86.8 us, 830 MB:
-    // 125.7 -> 124.9, 1107 MB: 166.5 -> 167.0; the mma.sync kernel gains 3 to 4 % at all three)
+    // 125.7 -> 124.9, 1107 MB: 166.5 -> 167.0; the mma.sync kernel gains 3 to 4 % at all three).  Page lists count as listed: rows
+    // of one sequence list some pages more than once, and still gain (4 sequences x 9 rows x 32 of 129 pages, 16 KV heads: 74.2 us
+    // against 76.3 without the hint, 75.0 / 76.7 where the rows' queries are alike; 2 x 9 rows of 250 pages 42.3 / 43.9).
     p.kv_read_once = (pl.row_groups == 1 && (long)a.batch * a.nkv * a.klen * 2 * a.cache_hd < (1024l << 20)) ? 1 : 0;
     p.block_table = a.block_table; p.seq_lens = a.seq_lens; p.max_pages = a.max_pages;
     p.unit_lists = a.unit_lists;

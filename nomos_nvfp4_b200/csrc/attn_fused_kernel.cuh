@@ -129,7 +129,8 @@ struct KParams {
                                     //    distributed shared memory (no partials in device memory, no arrival word)
     float *partial_export;          // optional exported (o, m, l) per row, m in natural-log units
     int early_rows;                 // window rows [0, early_rows) may be read before griddepcontrol.wait
-    int kv_read_once;               // 1: every cache byte is read by exactly one CTA of the launch (tile copies are marked evict-first in L2)
+    int kv_read_once;               // 1: tile copies are marked evict-first in L2: every cache byte is read by exactly one CTA of the launch (but
+                                    //    for pages that several query rows of a sequence list)
     // fused quantize-on-write: the last n_new keys of the window are given as fp32 rows
     const float *new_k, *new_v;     // [n_new][nkv][HD], row stride new_stride elements; nullptr = none
     uint8_t *k_cache_w, *v_cache_w, *k_scales_w, *v_scales_w;   // writable aliases of the cache
