@@ -491,8 +491,12 @@ int32_t nomos_kv_paged_page_bounds_i8(void *stream, uint64_t k_pool, uint64_t ks
  * that are not finite count as the largest finite value (a page of NaN keys is read, as dense attention would read it).
  * Every page but the row's last must have its bounds (see above).
  * sel_pages: 0, or [rows][nkv][top_pages], the page numbers within the sequence in ascending order, -1 beyond.
- * Accuracy of out: that of nomos_attn_paged_decode_i8 over the selected keys.  head_dim 128, at most 8 heads per KV head, at most
- * 2^30 rows.
+ * Accuracy of out: that of nomos_attn_paged_decode_i8 over the selected keys.  The query is taken as 16-bit fixed point of its row's
+ * largest element, also where it is fp32, so that a logit is off by up to  d = softmax_scale * max|q| * sum|k| / 63900 + 2^-19 *
+ * |logit|,  an absolute error that grows with the query, and an output by up to  sinh(d) e^d * (sum of weight * |v - out|)  for it;
+ * weights are rounded to 2^-17 of their page's largest.  Queries and keys of unit normal elements at softmax_scale 0.09: some 5e-5
+ * of the output's RMS; queries thirty times as large (logits in the hundreds): up to 2.5e-3.  head_dim 128, at most 8 heads per KV
+ * head, at most 2^30 rows.
  * The workspace (16-byte aligned) must not be shared by calls that can overlap on the GPU.  The bytes asked for `rows` also serve
  * every call of fewer rows, the other arguments alike. */
 int64_t nomos_attn_paged_sparse_workspace_bytes(int32_t rows, int32_t nh, int32_t nkv, int32_t kvg, int32_t l_hd, int32_t top_pages,
