@@ -512,7 +512,7 @@ typedef struct nomos_attn_sparse {
 int32_t nomos_attn_paged_sparse_i8(void *stream, const nomos_attn_sparse_t *args);
 /* Verification of drafted tokens from given random numbers.  Sequence b drafted n_draft[b] tokens (0 pointer: max_draft each;
  * negative: the sequence is idle and nothing of it is written; more than max_draft count as max_draft).  target_probs
- * [batch][max_draft + 1][p_stride], draft_probs [batch][max_draft][q_stride] fp32 rows of `vocab` probabilities in [0, 1]
+ * [batch][max_draft + 1][p_stride], draft_probs [batch][max_draft][q_stride] fp32 rows of `vocab` probabilities in [0, 1], their sum below 2^13
  * (draft_probs 0: a drafter that gives tokens only, probability 1 each); u_accept [batch][max_draft], u_sample [batch] in [0, 1).
  * Draft i of token x is accepted iff u_accept * q_i(x) < p_i(x), in 64 bits; a token outside [0, vocab) is rejected.  With a
  * the first one rejected (n_draft if none): n_accepted[b] = a, out_tokens [batch][max_draft + 1] = the a accepted tokens, then
