@@ -236,11 +236,11 @@ __global__ void __launch_bounds__(SV_THREADS, SV_CTAS_PER_SM) spec_verify_kernel
         for (int i = threadIdx.x; i <= a.max_draft; i += SV_THREADS)
             if (i != acc) a.out_tokens[(size_t)b * (a.max_draft + 1) + i] = i < acc ? a.tokens[(size_t)b * a.max_draft + i] : -1;
         if (threadIdx.x == 0) {
-            a.n_accepted[b] = acc;
-            if (a.lens) {                // (asked for again rather than kept in a register over the streams)
-                counts(other);
+            if (a.lens) {                // (asked for again rather than kept in a register over the streams; before n_accepted, which
+                counts(other);           // may lie over n_draft)
                 a.lens_out[b] = a.lens[b] + other + acc;
             }
+            a.n_accepted[b] = acc;
         }
     }
     cluster.sync();                      // the totals stay where the peers read them

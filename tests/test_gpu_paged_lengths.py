@@ -81,6 +81,23 @@ def test_granted_without_lengths_and_without_drafts():
     assert host(lens).tolist() == [130, 7, 9, 13]
 
 
+def test_accepted_counts_over_the_drafted_ones():
+    """n_accepted written over n_draft: lengths still follow from what was drafted."""
+    rng = np.random.default_rng(8)
+    batch, k, vocab = 40, 6, 500
+    z = 2 * rng.standard_normal((batch, k + 1, vocab))
+    p, q = softmax(z), softmax(z[:, :k] + 0.6 * rng.standard_normal((batch, k, vocab)))
+    tokens = np.argmax(q, -1)
+    n_draft, granted, lens = rng.integers(-1, k + 1, batch), rng.integers(0, 40, batch), rng.integers(0, 5000, batch)
+    ua, us = rng.random((batch, k), dtype=np.float32), rng.random(batch, dtype=np.float32)
+    dl, both, out = i32(lens), i32(n_draft), i32(np.full((batch, k + 1), -5))
+    ops.spec_verify(None, dev(p), dev(q), i32(tokens), both, dev(ua), dev(us), dl, dl, both, out, batch=batch, max_draft=k, vocab=vocab, p_stride=vocab, q_stride=vocab,
+                    granted=i32(granted))
+    torch.cuda.synchronize()
+    want = expected(p, q, tokens, n_draft, ua, us, granted, lens, n_draft, np.full((batch, k + 1), -5))
+    assert np.array_equal(host(dl), want[0]) and np.array_equal(host(both), want[1]) and np.array_equal(host(out), want[2])
+
+
 class Step:
     """The four calls as the integration notes list them, a request's length cleared when it ends; every launch of fixed size."""
 
